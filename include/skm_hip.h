@@ -49,6 +49,10 @@ int skm_device_count(int* out_count);
 
 /* One context = one device + one HIP stream + reusable workspace. */
 int skm_ctx_create(int device, skm_ctx** out_ctx);
+/* The same over a stream of the caller's (a hipStream_t of that device; null: the device's default stream), which has to
+ * outlive the context and stays the caller's: work of the context is ordered with the caller's own work on it, and a
+ * graph captured on it records the context's launches.  No counterpart in the reference. */
+int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx);
 int skm_ctx_destroy(skm_ctx* ctx);
 int skm_sync(skm_ctx* ctx);
 /* Upper bound, in bytes, of the scratch a single stage call may allocate (default 24 GiB of the
@@ -257,6 +261,85 @@ int skm_recall_hits(skm_ctx* ctx, const uint32_t* d_gt, const uint32_t* d_promis
  * bit for bit; d <= SKM_HOUSEHOLDER_Q_MAX_D (a workgroup keeps all rows of eight columns in LDS). */
 #define SKM_HOUSEHOLDER_Q_MAX_D 2272
 int skm_householder_q(skm_ctx* ctx, const double* h_a, size_t d, float* h_out_q);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators on rows of typed device tensors: what a table of centroids or embeddings needs next to the stages above where
+ * it is part of a model.  Rows looked up by id and the table's gradient (skm_gather_rows and skm_update for
+ * training), rows sorted by the groups a router chose and brought back with weights (skm_group_by_assignment for the k
+ * choices that skm_knn answers), rows quantised to 8 bits and products of them.  No counterpart in the reference.
+ *
+ *   - A value type is SKM_F32, SKM_F16 or SKM_BF16.  Sums are held in fp32 and rounded once, to nearest even.
+ *   - Matrices are row-major; a stride is the distance between rows in elements, at least the row length.  Any alignment to
+ *     the element's size serves; loads are 16 bytes wide where pointers, strides and row lengths allow.
+ *   - Outputs must not overlap inputs.  Elements between the rows of a strided output stay as they are.
+ *   - An index outside the rows it points into stands for no row (SKM_NO_ROW, which skm_knn leaves in empty slots, and
+ *     negative 64-bit ids among them): it is never followed.
+ *   - Calls allocate nothing, unless they take scratch and are given none: then it comes from the context's workspace,
+ *     which grows.  Scratch is device memory aligned to 16 bytes, of at least what the call's _scratch function says
+ *     for the same sizes; its contents before and after a call mean nothing, and no two calls that overlap in
+ *     time may share it.  A call captured into a graph that needs scratch has to be given it (SKM_ERR_INVALID
+ *     otherwise), as replays of two graphs would share the workspace.
+ *   - Results do not depend on the launch: no floating-point atomics, the same bits for the same call. */
+#define SKM_F32 0
+#define SKM_F16 1
+#define SKM_BF16 2
+#define SKM_U32 3 /* types of ids */
+#define SKM_I64 4
+#define SKM_NO_ROW 0xffffffffu
+#define SKM_ROW_MAX_D 1048576          /* longest row */
+#define SKM_ROUTE_MAX_CHOICES 1024     /* choices per row, as many as skm_knn answers */
+#define SKM_ROUTE_MAX_GROUPS 1048576
+#define SKM_ROUTE_MAX_PLACES 1073741824 /* rows * choices, or looked-up rows of a gradient */
+#define SKM_PRODUCT_MAX_K 131071       /* 128 * 128 * k stays below 2^31 */
+#define SKM_PRODUCT_MAX_M 1073741824
+#define SKM_PRODUCT_MAX_GROUPS 65536
+
+/* out[t] = scale * table[ids[t]] for t < n, a row of zeros where the id is no row of the table (rows x d).  ids_type:
+ * SKM_U32 or SKM_I64. */
+int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, size_t d, size_t table_stride, const void* d_ids,
+                    int ids_type, size_t n, float scale, void* d_out, size_t out_stride);
+/* Its gradient: out[v] = scale * (sum of grad[t] over the t with ids[t] == v), out (rows x d) of out_type, which is the
+ * gradient's type or SKM_F32.  accumulate != 0 adds that to what out holds and touches the rows that occur only; 0 writes every row, zeros
+ * where no token names it.  Tokens are added in an order that depends on the ids alone. */
+int skm_lookup_rows_grad_scratch(size_t n, size_t rows, size_t d, size_t* out_bytes);
+int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad_stride, const void* d_ids, int ids_type, size_t n,
+                         size_t rows, size_t d, float scale, void* d_out, int out_type, size_t out_stride, int accumulate,
+                         void* d_scratch, size_t scratch_bytes);
+
+/* Places of the n * choices choices (row-major, group numbers) in the stable order by group: slots[t][j] is the place of
+ * choice j of row t, order[p] the choice t * choices + j at place p, offsets[g] the first place of group g, and
+ * offsets[groups] the number of places in use.  A choice that is no group gets no place (SKM_NO_ROW); the entries of order
+ * behind the last place hold SKM_NO_ROW.  d_order (n * choices) may be null; d_offsets holds groups + 1 entries. */
+int skm_route_scratch(size_t n, size_t choices, size_t groups, size_t* out_bytes);
+int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices, size_t groups, uint32_t* d_slots,
+              uint32_t* d_order, uint32_t* d_offsets, void* d_scratch, size_t scratch_bytes);
+/* out[slots[t][j]] = x[t]: every row copied to its places.  Rows of out (out_rows x d) that are nobody's place stay as they are.
+ * Its gradient is skm_combine_rows without weights. */
+int skm_dispatch_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t d, size_t x_stride, const uint32_t* d_slots,
+                      size_t choices, void* d_out, size_t out_rows, size_t out_stride);
+/* out[t] = sum over j, ascending, of weights[t][j] * rows[slots[t][j]] (rows: n_rows x d; weights n x choices of weights_type,
+ * or null for ones).  A row without places is zeros. */
+int skm_combine_rows(skm_ctx* ctx, const void* d_rows, int type, size_t n_rows, size_t d, size_t rows_stride,
+                     const uint32_t* d_slots, size_t n, size_t choices, const void* d_weights, int weights_type, void* d_out,
+                     size_t out_stride);
+/* Its gradients: grad_rows[slots[t][j]] = weights[t][j] * grad[t] (rows that are nobody's place stay as they are) and
+ * grad_weights[t][j] = <grad[t], rows[slots[t][j]]> (of weights_type; 0 without a place).  Either output may be null; d_rows is
+ * read for the latter only.  Slots are distinct places, as skm_route makes them. */
+int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, size_t d, size_t grad_stride, const void* d_rows,
+                          size_t n_rows, size_t rows_stride, const uint32_t* d_slots, size_t choices, const void* d_weights,
+                          int weights_type, void* d_grad_rows, size_t grad_rows_stride, void* d_grad_weights);
+
+/* q[t][k] = the whole number nearest to 127 x[t][k] / max|x[t]|, ties to even, and scales[t] = max|x[t]| / 127.  A row of
+ * zeros has scale 0; a row that holds an infinity or NaN has scale NaN and q 0, so that its products are NaN. */
+int skm_quantize_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t d, size_t x_stride, int8_t* d_q, size_t q_stride,
+                      float* d_scales);
+/* out[i][j] = (sum over k of a[i][k] b[j][k]) * a_scale[i] * b_scale[j] + bias[j], out (m x n) of out_type; a is m x k, b is n x k.
+ * The sum is exact; d_bias may be null.  With d_offsets (groups + 1 entries, as skm_route makes them) the rows
+ * [offsets[g], offsets[g + 1]) of a are multiplied with the g-th matrix of b (b_group_stride elements apart), b_scale and bias
+ * (n apart), and rows of out that are in no group stay as they are.  Without, groups and b_group_stride are not looked at. */
+int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, const float* d_a_scale, const int8_t* d_b, size_t n,
+                   size_t k, size_t b_stride, const float* d_b_scale, const float* d_bias, size_t groups, size_t b_group_stride,
+                   const uint32_t* d_offsets, void* d_out, int out_type, size_t out_stride);
 
 /* Benchmark / test utility: seeded Gaussian-mixture rows generated in device memory.  Row i (logical
  * index row_offset + local row) is  s_j * (center_sigma * g(center_seed, u_i, j) + noise_sigma *

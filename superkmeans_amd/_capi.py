@@ -23,6 +23,7 @@ _PROTOTYPES = {
     "skm_last_error": (c_char_p, []),
     "skm_device_count": (c_int, [POINTER(c_int)]),
     "skm_ctx_create": (c_int, [c_int, POINTER(c_void_p)]),
+    "skm_ctx_create_on_stream": (c_int, [c_int, c_void_p, POINTER(c_void_p)]),
     "skm_ctx_destroy": (c_int, [c_void_p]),
     "skm_sync": (c_int, [c_void_p]),
     "skm_ctx_set_workspace_limit": (c_int, [c_void_p, c_size_t]),
@@ -102,6 +103,19 @@ _PROTOTYPES = {
         c_int, [c_void_p, c_size_t, c_void_p, c_size_t, POINTER(c_size_t), POINTER(c_size_t)]),
     "skm_dimension_split": (None, [c_size_t, POINTER(c_size_t), POINTER(c_size_t)]),
     "skm_pruner_tables": (c_int, [c_size_t, c_float, c_uint32, c_int, c_void_p, c_void_p]),
+    "skm_lookup_rows": (c_int, [c_void_p, _F, c_int, c_size_t, c_size_t, c_size_t, _F, c_int, c_size_t, c_float, _F, c_size_t]),
+    "skm_lookup_rows_grad_scratch": (c_int, [c_size_t, c_size_t, c_size_t, POINTER(c_size_t)]),
+    "skm_lookup_rows_grad": (c_int, [c_void_p, _F, c_int, c_size_t, _F, c_int, c_size_t, c_size_t, c_size_t, c_float, _F, c_int,
+                                     c_size_t, c_int, _F, c_size_t]),
+    "skm_route_scratch": (c_int, [c_size_t, c_size_t, c_size_t, POINTER(c_size_t)]),
+    "skm_route": (c_int, [c_void_p, _F, c_size_t, c_size_t, c_size_t, _F, _F, _F, _F, c_size_t]),
+    "skm_dispatch_rows": (c_int, [c_void_p, _F, c_int, c_size_t, c_size_t, c_size_t, _F, c_size_t, _F, c_size_t, c_size_t]),
+    "skm_combine_rows": (c_int, [c_void_p, _F, c_int, c_size_t, c_size_t, c_size_t, _F, c_size_t, c_size_t, _F, c_int, _F, c_size_t]),
+    "skm_combine_rows_grad": (c_int, [c_void_p, _F, c_int, c_size_t, c_size_t, c_size_t, _F, c_size_t, c_size_t, _F, c_size_t, _F,
+                                      c_int, _F, c_size_t, _F]),
+    "skm_quantize_rows": (c_int, [c_void_p, _F, c_int, c_size_t, c_size_t, c_size_t, _F, c_size_t, _F]),
+    "skm_product_i8": (c_int, [c_void_p, _F, c_size_t, c_size_t, _F, _F, c_size_t, c_size_t, c_size_t, _F, _F, c_size_t, c_size_t,
+                               _F, _F, c_int, c_size_t]),
 }
 
 
@@ -232,12 +246,20 @@ class DeviceArray:
 
 
 class Context:
-    """One device + stream + workspace (skm_ctx)."""
+    """One device + stream + workspace (skm_ctx).
 
-    def __init__(self, device=0):
+    `stream`: None for a stream of its own, or the handle of a stream to work on (an integer, 0 for the device's default
+    stream), which has to outlive the context.
+    """
+
+    def __init__(self, device=0, stream=None):
         self.lib = load()
         h = c_void_p()
-        check(self.lib.skm_ctx_create(device, ctypes.byref(h)))
+        self.handle = None
+        if stream is None:
+            check(self.lib.skm_ctx_create(device, ctypes.byref(h)))
+        else:
+            check(self.lib.skm_ctx_create_on_stream(device, c_void_p(stream), ctypes.byref(h)))
         self.handle = h.value
         self._live = []
 

@@ -1,0 +1,389 @@
+// Rows of a table looked up by id, rows sent to their groups and brought back with weights, and the gradients of the
+// latter.  All of it moves rows: the bytes of the rows bound every kernel here, and the arithmetic is a product and a sum
+// per element.
+#include "rows_common.h"
+
+namespace skm {
+
+int call_scratch(skm_ctx* ctx, const char* who, void* given, const size_t given_bytes, const size_t need, void** out) {
+    if (need == 0) {
+        *out = nullptr;
+        return SKM_OK;
+    }
+    if (given) {
+        if (given_bytes < need)
+            return set_error(SKM_ERR_INVALID, "%s: %zu bytes of scratch given, %zu needed", who, given_bytes, need);
+        if (address(given) % 16) return set_error(SKM_ERR_INVALID, "%s: scratch must be 16-byte aligned", who);
+        *out = given;
+        return SKM_OK;
+    }
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    SKM_HIP_TRY(hipStreamIsCapturing(ctx->stream, &status));
+    if (status != hipStreamCaptureStatusNone)
+        return set_error(SKM_ERR_INVALID, "%s: a captured call brings its own scratch", who);
+    if (need > ctx->workspace_limit)
+        return set_error(SKM_ERR_INVALID, "%s: %zu bytes of scratch needed, the workspace limit is %zu", who, need,
+                         ctx->workspace_limit);
+    return workspace(ctx, skm_ctx::WS_ROWS, need, out);
+}
+
+namespace {
+
+constexpr int UNROLL = 4;  // vectors a lane requests before it uses the first
+
+// id of position i, or a number at or past every table size where there is none
+__device__ __forceinline__ uint64_t id_at(const void* ids, const int ids_type, const size_t i) {
+    return ids_type == SKM_I64 ? reinterpret_cast<const uint64_t*>(ids)[i] : (uint64_t) reinterpret_cast<const uint32_t*>(ids)[i];
+}
+
+// out[t] = scale * table[id_t], a row of zeros where the id is no row.  A lane requests UNROLL vectors of its row before
+// it stores the first.
+template <class T, int E>
+__global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
+    const T* __restrict__ table, const size_t rows, const size_t table_stride, const void* __restrict__ ids, const int ids_type,
+    const size_t n, const float scale, T* __restrict__ out, const size_t out_stride, const RowSplit s
+) {
+    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
+    const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
+    for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
+        const size_t t = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
+        if (t >= n) continue;
+        const uint32_t first = (uint32_t) (u % s.pieces) * s.lanes * UNROLL + in_row;
+        const uint64_t id = id_at(ids, ids_type, t);
+        const bool there = id < rows;
+        const T* from = table + (there ? id : 0) * table_stride;
+        T* to = out + t * out_stride;
+        vec_of<T, E> v[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const uint32_t at = first + i * s.lanes;
+            if (at < s.vectors && there) v[i] = load_vec<T, E>(from + (size_t) at * E);
+        }
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const uint32_t at = first + i * s.lanes;
+            if (at < s.vectors) {
+                vec_of<T, E> r = {};
+                if (there) r = scale == 1.0f ? v[i] : narrow<T, E>(widen<E>(v[i]) * scale);
+                store_vec<T, E>(to + (size_t) at * E, r);
+            }
+        }
+    }
+}
+
+// out[slot[t][j]] = x[t] for every choice j that has a slot: the row is read once and stored once per choice.
+template <class T, int E>
+__global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
+    const T* __restrict__ x, const size_t x_stride, const size_t n, const uint32_t* __restrict__ slots, const uint32_t choices,
+    const size_t out_rows, T* __restrict__ out, const size_t out_stride, const RowSplit s
+) {
+    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
+    const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
+    for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
+        const size_t t = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
+        if (t >= n) continue;
+        const uint32_t first = (uint32_t) (u % s.pieces) * s.lanes * UNROLL + in_row;
+        vec_of<T, E> v[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) {
+            const uint32_t at = first + i * s.lanes;
+            if (at < s.vectors) v[i] = load_vec<T, E>(x + t * x_stride + (size_t) at * E);
+        }
+        for (uint32_t j = 0; j < choices; ++j) {
+            const uint32_t slot = slots[t * choices + j];
+            if (slot >= out_rows) continue;
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i) {
+                const uint32_t at = first + i * s.lanes;
+                if (at < s.vectors) store_vec<T, E>(out + (size_t) slot * out_stride + (size_t) at * E, v[i]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float weight_at(const void* weights, const int type, const size_t i) {
+    if (type == SKM_F32) return reinterpret_cast<const float*>(weights)[i];
+    if (type == SKM_F16) return (float) reinterpret_cast<const _Float16*>(weights)[i];
+    return (float) reinterpret_cast<const __bf16*>(weights)[i];
+}
+__device__ __forceinline__ void put_weight(void* weights, const int type, const size_t i, const float v) {
+    if (type == SKM_F32) reinterpret_cast<float*>(weights)[i] = v;
+    else if (type == SKM_F16) reinterpret_cast<_Float16*>(weights)[i] = (_Float16) v;
+    else reinterpret_cast<__bf16*>(weights)[i] = (__bf16) v;
+}
+
+constexpr int COMBINE_UNROLL = 2;  // vectors per lane
+constexpr int COMBINE_AHEAD = 4;   // choices whose rows are requested together
+
+// out[t] = sum_j w[t][j] * rows[slot[t][j]], j ascending, in fp32.
+template <class T, int E>
+__global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
+    const T* __restrict__ rows, const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const size_t n,
+    const uint32_t choices, const void* __restrict__ weights, const int weights_type, T* __restrict__ out, const size_t out_stride,
+    const RowSplit s
+) {
+    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
+    const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
+    for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
+        const size_t t = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
+        if (t >= n) continue;
+        const uint32_t first = (uint32_t) (u % s.pieces) * s.lanes * COMBINE_UNROLL + in_row;
+        vec_of<float, E> sum[COMBINE_UNROLL] = {};
+        for (uint32_t j0 = 0; j0 < choices; j0 += COMBINE_AHEAD) {
+            vec_of<T, E> v[COMBINE_AHEAD][COMBINE_UNROLL];
+            uint32_t slot[COMBINE_AHEAD];
+            float w[COMBINE_AHEAD];
+#pragma unroll
+            for (int j = 0; j < COMBINE_AHEAD; ++j) {
+                slot[j] = j0 + j < choices ? slots[t * choices + j0 + j] : SKM_NO_ROW;
+                w[j] = 1.0f;
+                if (weights && slot[j] < n_rows) w[j] = weight_at(weights, weights_type, t * choices + j0 + j);
+            }
+#pragma unroll
+            for (int j = 0; j < COMBINE_AHEAD; ++j)
+#pragma unroll
+                for (int i = 0; i < COMBINE_UNROLL; ++i) {
+                    const uint32_t at = first + i * s.lanes;
+                    if (slot[j] < n_rows && at < s.vectors)
+                        v[j][i] = load_vec<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                }
+#pragma unroll
+            for (int j = 0; j < COMBINE_AHEAD; ++j)
+                if (slot[j] < n_rows)
+#pragma unroll
+                    for (int i = 0; i < COMBINE_UNROLL; ++i) sum[i] += w[j] * widen<E>(v[j][i]);
+        }
+#pragma unroll
+        for (int i = 0; i < COMBINE_UNROLL; ++i) {
+            const uint32_t at = first + i * s.lanes;
+            if (at < s.vectors) store_vec<T, E>(out + t * out_stride + (size_t) at * E, narrow<T, E>(sum[i]));
+        }
+    }
+}
+
+constexpr int GRAD_CHOICES = 8;  // choices whose products are summed in one walk over the row
+
+// grad_rows[slot[t][j]] = w[t][j] * grad[t] and grad_w[t][j] = <grad[t], rows[slot[t][j]]>: one walk over the token's row
+// for each GRAD_CHOICES choices, WAVES wavefronts per token.
+template <class T, int E, int WAVES>
+__global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
+    const T* __restrict__ grad, const size_t n, const uint32_t vectors, const size_t grad_stride, const T* __restrict__ rows,
+    const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const uint32_t choices,
+    const void* __restrict__ weights, const int weights_type, T* __restrict__ grad_rows, const size_t grad_rows_stride,
+    void* __restrict__ grad_weights
+) {
+    constexpr int TOKENS = ROWS_THREADS / 64 / WAVES;  // tokens per workgroup
+    __shared__ float part[ROWS_THREADS / 64][GRAD_CHOICES];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t in_row = threadIdx.x % (64 * WAVES);
+    // every thread of a workgroup takes the same number of turns, so that all of them meet at the barriers
+    const size_t turns = (n + TOKENS - 1) / TOKENS;
+    for (size_t turn = blockIdx.x; turn < turns; turn += gridDim.x) {
+        const size_t t = turn * TOKENS + wave / WAVES;
+        for (uint32_t j0 = 0; j0 < choices; j0 += GRAD_CHOICES) {
+            float dot[GRAD_CHOICES] = {};
+            if (t < n) {
+                uint32_t slot[GRAD_CHOICES];
+                float w[GRAD_CHOICES];
+#pragma unroll
+                for (int j = 0; j < GRAD_CHOICES; ++j) {
+                    slot[j] = j0 + j < choices ? slots[t * choices + j0 + j] : SKM_NO_ROW;
+                    w[j] = 1.0f;
+                    if (weights && slot[j] < n_rows) w[j] = weight_at(weights, weights_type, t * choices + j0 + j);
+                }
+                for (uint32_t at = in_row; at < vectors; at += 64 * WAVES) {
+                    const vec_of<float, E> g = widen<E>(load_vec<T, E>(grad + t * grad_stride + (size_t) at * E));
+                    vec_of<T, E> y[GRAD_CHOICES];
+                    if (grad_weights) {
+#pragma unroll
+                        for (int j = 0; j < GRAD_CHOICES; ++j)
+                            if (slot[j] < n_rows) y[j] = load_vec<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                    }
+#pragma unroll
+                    for (int j = 0; j < GRAD_CHOICES; ++j) {
+                        if (slot[j] >= n_rows) continue;
+                        if (grad_weights) {
+                            const vec_of<float, E> p = g * widen<E>(y[j]);
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int e = 0; e < E; ++e) sum += p[e];
+                            dot[j] += sum;
+                        }
+                        if (grad_rows)
+                            store_vec<T, E>(grad_rows + (size_t) slot[j] * grad_rows_stride + (size_t) at * E, narrow<T, E>(g * w[j]));
+                    }
+                }
+            }
+            if (grad_weights) {
+#pragma unroll
+                for (int j = 0; j < GRAD_CHOICES; ++j)
+#pragma unroll
+                    for (int off = 32; off > 0; off >>= 1) dot[j] += __shfl_xor(dot[j], off);
+                if (WAVES == 1) {
+                    if (t < n && lane == 0)
+#pragma unroll
+                        for (int j = 0; j < GRAD_CHOICES; ++j)
+                            if (j0 + j < choices) put_weight(grad_weights, weights_type, t * choices + j0 + j, dot[j]);
+                } else {
+                    __syncthreads();  // the sums of the turn before have been read
+                    if (lane == 0)
+#pragma unroll
+                        for (int j = 0; j < GRAD_CHOICES; ++j) part[wave][j] = dot[j];
+                    __syncthreads();
+                    if (t < n && in_row < GRAD_CHOICES && j0 + in_row < choices) {
+                        float sum = 0.0f;
+                        for (int i = 0; i < WAVES; ++i) sum += part[wave / WAVES * WAVES + i][in_row];
+                        put_weight(grad_weights, weights_type, t * choices + j0 + in_row, sum);
+                    }
+                }
+            }
+        }
+    }
+}
+
+} // namespace
+} // namespace skm
+
+using namespace skm;
+
+extern "C" {
+
+int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, size_t d, size_t table_stride, const void* d_ids,
+                    int ids_type, size_t n, float scale, void* d_out, size_t out_stride) {
+    SKM_REQUIRE(ctx, "null context");
+    SKM_REQUIRE(is_value_type(type), "type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE(ids_type == SKM_U32 || ids_type == SKM_I64, "ids_type must be SKM_U32 or SKM_I64");
+    SKM_REQUIRE(d > 0 && d <= SKM_ROW_MAX_D, "d out of range");
+    SKM_REQUIRE(table_stride >= d && out_stride >= d, "strides must be at least d");
+    SKM_REQUIRE(rows < SKM_NO_ROW && n < SKM_NO_ROW, "rows and n must fit in 32 bits");
+    if (n == 0) return SKM_OK;
+    SKM_REQUIRE(d_ids && d_out && (d_table || rows == 0), "null pointer");
+    const size_t size = type_size(type);
+    SKM_REQUIRE(address(d_ids) % (ids_type == SKM_I64 ? 8 : 4) == 0 && address(d_table) % size == 0 && address(d_out) % size == 0,
+                "pointers must be aligned to their elements");
+    SKM_REQUIRE(!overlap(d_table, span(rows, table_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the table");
+    OnDevice on(ctx);
+    ScopedStage st(ctx, "rows/lookup");
+    const size_t width = common_width({address(d_table), address(d_out), table_stride * size, out_stride * size, d * size});
+    return for_type(type, [&](auto sample) {
+        using T = decltype(sample);
+        return for_width<T>(width, [&](auto elements) {
+            constexpr int E = decltype(elements)::value;
+            const RowSplit s = split_rows(n, d / E, UNROLL);
+            lookup_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
+                (const T*) d_table, rows, table_stride, d_ids, ids_type, n, scale, (T*) d_out, out_stride, s);
+            return check_hip(hipGetLastError(), "lookup_rows_kernel launch");
+        });
+    });
+}
+
+int skm_dispatch_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t d, size_t x_stride, const uint32_t* d_slots,
+                      size_t choices, void* d_out, size_t out_rows, size_t out_stride) {
+    SKM_REQUIRE(ctx, "null context");
+    SKM_REQUIRE(is_value_type(type), "type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE(d > 0 && d <= SKM_ROW_MAX_D, "d out of range");
+    SKM_REQUIRE(x_stride >= d && out_stride >= d, "strides must be at least d");
+    SKM_REQUIRE(n < SKM_NO_ROW && out_rows < SKM_NO_ROW, "row counts must fit in 32 bits");
+    SKM_REQUIRE(choices > 0 && choices <= SKM_ROUTE_MAX_CHOICES, "choices out of range");
+    if (n == 0 || out_rows == 0) return SKM_OK;
+    SKM_REQUIRE(d_x && d_slots && d_out, "null pointer");
+    const size_t size = type_size(type);
+    SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_x) % size == 0 && address(d_out) % size == 0,
+                "pointers must be aligned to their elements");
+    SKM_REQUIRE(!overlap(d_x, span(n, x_stride, d, size), d_out, span(out_rows, out_stride, d, size)), "out overlaps x");
+    OnDevice on(ctx);
+    ScopedStage st(ctx, "rows/dispatch");
+    const size_t width = common_width({address(d_x), address(d_out), x_stride * size, out_stride * size, d * size});
+    return for_type(type, [&](auto sample) {
+        using T = decltype(sample);
+        return for_width<T>(width, [&](auto elements) {
+            constexpr int E = decltype(elements)::value;
+            const RowSplit s = split_rows(n, d / E, UNROLL);
+            dispatch_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
+                (const T*) d_x, x_stride, n, d_slots, (uint32_t) choices, out_rows, (T*) d_out, out_stride, s);
+            return check_hip(hipGetLastError(), "dispatch_rows_kernel launch");
+        });
+    });
+}
+
+int skm_combine_rows(skm_ctx* ctx, const void* d_rows, int type, size_t n_rows, size_t d, size_t rows_stride,
+                     const uint32_t* d_slots, size_t n, size_t choices, const void* d_weights, int weights_type, void* d_out,
+                     size_t out_stride) {
+    SKM_REQUIRE(ctx, "null context");
+    SKM_REQUIRE(is_value_type(type), "type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE(!d_weights || is_value_type(weights_type), "weights_type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE(d > 0 && d <= SKM_ROW_MAX_D, "d out of range");
+    SKM_REQUIRE(rows_stride >= d && out_stride >= d, "strides must be at least d");
+    SKM_REQUIRE(n < SKM_NO_ROW && n_rows < SKM_NO_ROW, "row counts must fit in 32 bits");
+    SKM_REQUIRE(choices > 0 && choices <= SKM_ROUTE_MAX_CHOICES, "choices out of range");
+    if (n == 0) return SKM_OK;
+    SKM_REQUIRE((d_rows || n_rows == 0) && d_slots && d_out, "null pointer");
+    const size_t size = type_size(type);
+    SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_rows) % size == 0 && address(d_out) % size == 0 &&
+                (!d_weights || address(d_weights) % type_size(weights_type) == 0), "pointers must be aligned to their elements");
+    SKM_REQUIRE(!overlap(d_rows, span(n_rows, rows_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the rows");
+    OnDevice on(ctx);
+    ScopedStage st(ctx, "rows/combine");
+    const size_t width = common_width({address(d_rows), address(d_out), rows_stride * size, out_stride * size, d * size});
+    return for_type(type, [&](auto sample) {
+        using T = decltype(sample);
+        return for_width<T>(width, [&](auto elements) {
+            constexpr int E = decltype(elements)::value;
+            const RowSplit s = split_rows(n, d / E, COMBINE_UNROLL);
+            combine_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
+                (const T*) d_rows, n_rows, rows_stride, d_slots, n, (uint32_t) choices, d_weights, weights_type, (T*) d_out,
+                out_stride, s);
+            return check_hip(hipGetLastError(), "combine_rows_kernel launch");
+        });
+    });
+}
+
+int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, size_t d, size_t grad_stride, const void* d_rows,
+                          size_t n_rows, size_t rows_stride, const uint32_t* d_slots, size_t choices, const void* d_weights,
+                          int weights_type, void* d_grad_rows, size_t grad_rows_stride, void* d_grad_weights) {
+    SKM_REQUIRE(ctx, "null context");
+    SKM_REQUIRE(is_value_type(type), "type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE((!d_weights && !d_grad_weights) || is_value_type(weights_type), "weights_type must be SKM_F32, SKM_F16 or SKM_BF16");
+    SKM_REQUIRE(d > 0 && d <= SKM_ROW_MAX_D, "d out of range");
+    SKM_REQUIRE(grad_stride >= d && (!d_grad_weights || rows_stride >= d) && (!d_grad_rows || grad_rows_stride >= d),
+                "strides must be at least d");
+    SKM_REQUIRE(n < SKM_NO_ROW && n_rows < SKM_NO_ROW, "row counts must fit in 32 bits");
+    SKM_REQUIRE(choices > 0 && choices <= SKM_ROUTE_MAX_CHOICES, "choices out of range");
+    SKM_REQUIRE(d_grad_rows || d_grad_weights, "no output asked for");
+    if (n == 0) return SKM_OK;
+    SKM_REQUIRE(d_grad && d_slots && (d_rows || !d_grad_weights || n_rows == 0), "null pointer");
+    const size_t size = type_size(type), weight_size = type_size(weights_type);
+    SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_grad) % size == 0 && address(d_rows) % size == 0 &&
+                address(d_grad_rows) % size == 0 && (!d_weights || address(d_weights) % weight_size == 0) &&
+                (!d_grad_weights || address(d_grad_weights) % weight_size == 0), "pointers must be aligned to their elements");
+    if (d_grad_rows) {
+        const size_t bytes = span(n_rows, grad_rows_stride, d, size);
+        SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps grad");
+        SKM_REQUIRE(!d_grad_weights || !overlap(d_rows, span(n_rows, rows_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps the rows");
+    }
+    OnDevice on(ctx);
+    ScopedStage st(ctx, "rows/combine_grad");
+    size_t width = common_width({address(d_grad), grad_stride * size, d * size});
+    if (d_grad_weights) width = std::min(width, common_width({address(d_rows), rows_stride * size}));
+    if (d_grad_rows) width = std::min(width, common_width({address(d_grad_rows), grad_rows_stride * size}));
+    return for_type(type, [&](auto sample) {
+        using T = decltype(sample);
+        return for_width<T>(width, [&](auto elements) {
+            constexpr int E = decltype(elements)::value;
+            const uint32_t vectors = (uint32_t) (d / E);
+            const auto launch = [&](auto waves) {
+                constexpr int WAVES = decltype(waves)::value;
+                const size_t turns = (n + ROWS_THREADS / 64 / WAVES - 1) / (ROWS_THREADS / 64 / WAVES);
+                const unsigned blocks = (unsigned) std::min<uint64_t>(ROWS_MAX_BLOCKS, turns);
+                combine_rows_grad_kernel<T, E, WAVES><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
+                    (const T*) d_grad, n, vectors, grad_stride, (const T*) d_rows, n_rows, rows_stride, d_slots, (uint32_t) choices,
+                    d_weights, weights_type, (T*) d_grad_rows, grad_rows_stride, d_grad_weights);
+                return check_hip(hipGetLastError(), "combine_rows_grad_kernel launch");
+            };
+            if (vectors > 64) return launch(std::integral_constant<int, 4>{});
+            return launch(std::integral_constant<int, 1>{});
+        });
+    });
+}
+
+} // extern "C"

@@ -1,0 +1,137 @@
+// What the operators on rows of typed device tensors share: element types, vectors of them, the split of rows over
+// wavefronts, and the checks of their entry points.
+#pragma once
+
+#include "skm_internal.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace skm {
+
+template <class T, int N>
+using vec_of = T __attribute__((ext_vector_type(N)));
+
+// Sums are held in fp32; a result is rounded once, to nearest even, when it is stored.
+template <int N, class T>
+__device__ __forceinline__ vec_of<float, N> widen(const vec_of<T, N> v) {
+    return __builtin_convertvector(v, vec_of<float, N>);
+}
+template <class T, int N>
+__device__ __forceinline__ vec_of<T, N> narrow(const vec_of<float, N> v) {
+    return __builtin_convertvector(v, vec_of<T, N>);
+}
+
+// Vectors of at most 16 bytes for results that are wider than their inputs.
+template <class T, int N>
+__device__ __forceinline__ void store_vec(T* p, const vec_of<T, N> v) {
+    if constexpr (sizeof(T) * N <= 16) {
+        *reinterpret_cast<vec_of<T, N>*>(p) = v;
+    } else {
+        constexpr int H = N / 2;
+        vec_of<T, H> lo, hi;
+#pragma unroll
+        for (int i = 0; i < H; ++i) lo[i] = v[i], hi[i] = v[H + i];
+        store_vec<T, H>(p, lo);
+        store_vec<T, H>(p + H, hi);
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ vec_of<T, N> load_vec(const T* p) {
+    if constexpr (sizeof(T) * N <= 16) {
+        return *reinterpret_cast<const vec_of<T, N>*>(p);
+    } else {
+        constexpr int H = N / 2;
+        const vec_of<T, H> lo = load_vec<T, H>(p), hi = load_vec<T, H>(p + H);
+        vec_of<T, N> v;
+#pragma unroll
+        for (int i = 0; i < H; ++i) v[i] = lo[i], v[H + i] = hi[i];
+        return v;
+    }
+}
+
+inline size_t type_size(const int type) { return type == SKM_F32 ? 4 : 2; }
+inline bool is_value_type(const int type) { return type == SKM_F32 || type == SKM_F16 || type == SKM_BF16; }
+
+// Largest power of two of at most 16 that divides all of the given byte counts and addresses: the width of a load.
+inline size_t common_width(std::initializer_list<size_t> of) {
+    size_t all = 16;
+    for (const size_t v : of) all |= v;
+    return all & (~all + 1);
+}
+inline size_t address(const void* p) { return reinterpret_cast<size_t>(p); }
+
+inline bool overlap(const void* a, const size_t a_bytes, const void* b, const size_t b_bytes) {
+    return a && b && address(a) < address(b) + b_bytes && address(b) < address(a) + a_bytes;
+}
+// Bytes from the first to the last element of a matrix.
+inline size_t span(const size_t rows, const size_t stride, const size_t d, const size_t size) {
+    return rows ? ((rows - 1) * stride + d) * size : 0;
+}
+
+// The calling thread's device is the context's while an entry point launches, and what it was afterwards (the default
+// stream, which a context may be made on, belongs to the current device).
+class OnDevice {
+  public:
+    explicit OnDevice(const skm_ctx* ctx) {
+        if (hipGetDevice(&before_) != hipSuccess) before_ = ctx->device;
+        if (before_ != ctx->device) switched_ = hipSetDevice(ctx->device) == hipSuccess;
+    }
+    ~OnDevice() {
+        if (switched_) (void) hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+  private:
+    int before_ = 0;
+    bool switched_ = false;
+};
+
+// Scratch of a call: the caller's block, or the context's workspace where none is given.  The workspace may grow, which
+// allocates and waits, and two graphs captured on one context would share it: under capture the caller brings the block.
+int call_scratch(skm_ctx* ctx, const char* who, void* given, size_t given_bytes, size_t need, void** out);
+
+// How rows are handed out.  A wavefront takes `lanes` lanes per row (a power of two) and so 64 / lanes rows at a time; a
+// row of more than lanes * UNROLL vectors is cut into pieces that different wavefronts take.
+struct RowSplit {
+    uint32_t vectors;  // vectors per row
+    uint32_t lanes;
+    uint32_t pieces;   // pieces per row
+    uint64_t units;    // wavefronts' worth of work: groups of 64 / lanes rows times pieces
+};
+inline RowSplit split_rows(const size_t n, const size_t vectors, const uint32_t unroll) {
+    RowSplit s;
+    s.vectors = (uint32_t) vectors;
+    s.lanes = 1;
+    while (s.lanes < 64 && (size_t) s.lanes * unroll < vectors) s.lanes *= 2;
+    const size_t per_piece = (size_t) s.lanes * unroll;
+    s.pieces = (uint32_t) ((vectors + per_piece - 1) / per_piece);
+    const size_t rows_per_wave = 64 / s.lanes;
+    s.units = (uint64_t) ((n + rows_per_wave - 1) / rows_per_wave) * s.pieces;
+    return s;
+}
+constexpr int ROWS_THREADS = 256;
+constexpr uint64_t ROWS_MAX_BLOCKS = uint64_t(1) << 22;  // beyond that a wavefront takes several units
+inline unsigned row_blocks(const RowSplit& s) {
+    const uint64_t per_block = ROWS_THREADS / 64;
+    return (unsigned) std::max<uint64_t>(1, std::min(ROWS_MAX_BLOCKS, (s.units + per_block - 1) / per_block));
+}
+
+// Calls f with a value of the element type, and with the vector width in elements, that a call's types and alignment ask for.
+template <class F>
+int for_type(const int type, F&& f) {
+    if (type == SKM_F32) return f(float{});
+    if (type == SKM_F16) return f(_Float16{});
+    return f(__bf16{});
+}
+template <class T, class F>
+int for_width(const size_t bytes, F&& f) {
+    if (bytes >= 16) return f(std::integral_constant<int, 16 / sizeof(T)>{});
+    if (bytes >= 8) return f(std::integral_constant<int, 8 / sizeof(T)>{});
+    if constexpr (sizeof(T) == 2)
+        if (bytes >= 4) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 1>{});
+}
+
+} // namespace skm

@@ -263,7 +263,7 @@ int skm_device_count(int* out_count) {
     return SKM_OK;
 }
 
-int skm_ctx_create(int device, skm_ctx** out_ctx) {
+static int create_context(int device, bool own_stream, void* stream, skm_ctx** out_ctx) {
     if (!out_ctx) return set_error(SKM_ERR_INVALID, "skm_ctx_create: null output");
     *out_ctx = nullptr;
     int n = 0;
@@ -282,21 +282,32 @@ int skm_ctx_create(int device, skm_ctx** out_ctx) {
     skm_ctx* ctx = new skm_ctx();
     ctx->device = device;
     ctx->noalloc_scratch = noalloc_scratch;
-    hipError_t e = hipStreamCreate(&ctx->stream);
-    if (e != hipSuccess) {
-        delete ctx;
-        return check_hip(e, "hipStreamCreate");
+    ctx->owns_stream = own_stream;
+    if (own_stream) {
+        const hipError_t e = hipStreamCreate(&ctx->stream);
+        if (e != hipSuccess) {
+            delete ctx;
+            return check_hip(e, "hipStreamCreate");
+        }
+    } else {
+        ctx->stream = (hipStream_t) stream;
     }
     // The pinned block is made here rather than at its first use, which falls into the middle of an iteration:
     // pinning host memory while kernels run holds them up (helper contexts are created while the device is idle).
     const int rc = pinned_block(ctx);
     if (rc != SKM_OK) {
-        (void) hipStreamDestroy(ctx->stream);
+        if (own_stream) (void) hipStreamDestroy(ctx->stream);
         delete ctx;
         return rc;
     }
     *out_ctx = ctx;
     return SKM_OK;
+}
+
+int skm_ctx_create(int device, skm_ctx** out_ctx) { return create_context(device, true, nullptr, out_ctx); }
+
+int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx) {
+    return create_context(device, false, stream, out_ctx);
 }
 
 int skm_ctx_destroy(skm_ctx* ctx) {
@@ -322,7 +333,7 @@ int skm_ctx_destroy(skm_ctx* ctx) {
             if (e) (void) hipEventDestroy(e);
         (void) hipStreamDestroy(ctx->copy_stream);
     }
-    (void) hipStreamDestroy(ctx->stream);
+    if (ctx->owns_stream) (void) hipStreamDestroy(ctx->stream);
     delete ctx;
     return SKM_OK;
 }

@@ -23,6 +23,7 @@ struct skm_pending_interval {
 struct skm_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool owns_stream = true;  // false: the caller's (skm_ctx_create_on_stream)
     // Transfer stream of skm_upload_overlapped (created on first use) and the events that order it before `stream`.
     hipStream_t copy_stream = nullptr;
     hipEvent_t copy_done[8] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
@@ -33,9 +34,10 @@ struct skm_ctx {
     int walk_launches = 1;     // skm_ctx_set_walk_launches
     uint64_t last_overflow_points = 0;  // skm_ctx_get_last_overflow
     // Grow-only scratch buffers, one per role, so that stages never free inside a hot loop.
-    static constexpr int WS_SLOTS = 6;
-    void* ws[WS_SLOTS] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-    size_t ws_bytes[WS_SLOTS] = {0, 0, 0, 0, 0, 0};
+    static constexpr int WS_SLOTS = 7;
+    static constexpr int WS_ROWS = 6;  // the operators on rows of typed tensors
+    void* ws[WS_SLOTS] = {};
+    size_t ws_bytes[WS_SLOTS] = {};
     // Point ids grouped by assignment, as the last centroid update sorted them (workspace slot 4, valid for
     // cluster_order_n points).  The pruned search visits the points in this order: neighbours in it share their
     // centroid row and most of their candidate blocks, which then come from the cache of the compute die that

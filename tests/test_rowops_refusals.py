@@ -1,0 +1,165 @@
+"""What superkmeans_amd.rowops refuses before anything reaches a device (no GPU needed).
+
+The tensors here have the attributes of device tensors and no memory; the context's library is a stand-in that records the
+calls which would have been made.
+"""
+import pytest
+
+from superkmeans_amd import rowops
+
+
+class Device:
+    def __init__(self, type="cuda", index=0):
+        self.type, self.index = type, index
+
+    def __str__(self):
+        return f"{self.type}:{self.index}"
+
+
+class Tensor:
+    def __init__(self, shape, dtype="float32", stride=None, device=Device(), at=0x1000):
+        self.shape, self.dtype, self.device, self._at = tuple(shape), f"torch.{dtype}", device, at
+        if stride is None:
+            stride, step = [], 1
+            for size in reversed(self.shape):
+                stride.insert(0, step)
+                step *= max(size, 1)
+        self._stride = tuple(stride)
+
+    def stride(self):
+        return self._stride
+
+    def data_ptr(self):
+        return self._at
+
+
+class Library:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+class Context:
+    def __init__(self):
+        self.lib, self.handle = Library(), 1
+
+
+@pytest.fixture
+def ops():
+    o = rowops.RowOperators(ctx=Context())
+    yield o
+    o.close()
+
+
+T, I = Tensor, lambda shape, **kw: Tensor(shape, "int32", **kw)
+
+
+def q8(shape, **kw):
+    return Tensor(shape, "int8", **kw)
+
+
+BAD = {
+    "lookup out of another type": lambda o: o.lookup(T((9, 4)), I((3,)), T((3, 4), "bfloat16")),
+    "lookup out of another shape": lambda o: o.lookup(T((9, 4)), I((3,)), T((4, 4))),
+    "lookup table of an integer type": lambda o: o.lookup(I((9, 4)), I((3,)), I((3, 4))),
+    "lookup ids of a float type": lambda o: o.lookup(T((9, 4)), T((3,)), T((3, 4))),
+    "lookup ids of two dimensions": lambda o: o.lookup(T((9, 4)), I((3, 1)), T((3, 4))),
+    "lookup ids with gaps": lambda o: o.lookup(T((9, 4)), I((3,), stride=(2,)), T((3, 4))),
+    "lookup table by columns": lambda o: o.lookup(T((9, 4), stride=(1, 9)), I((3,)), T((3, 4))),
+    "lookup table broadcast": lambda o: o.lookup(T((9, 4), stride=(0, 1)), I((3,)), T((3, 4))),
+    "lookup out on the host": lambda o: o.lookup(T((9, 4)), I((3,)), T((3, 4), device=Device("cpu", None))),
+    "lookup table on another device": lambda o: o.lookup(T((9, 4), device=Device("cuda", 1)), I((3,)), T((3, 4))),
+    "lookup of a list": lambda o: o.lookup([[1.0]], I((3,)), T((3, 4))),
+    "gradient with too few ids": lambda o: o.lookup_grad(T((3, 4)), I((2,)), T((9, 4))),
+    "gradient into half precision": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 4), "float16")),
+    "gradient between half types": lambda o: o.lookup_grad(T((3, 4), "bfloat16"), I((3,)), T((9, 4), "float16")),
+    "gradient of other columns": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 5))),
+    "gradient with a matrix of scratch": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 4)), scratch=T((9, 9))),
+    "route of 64-bit choices": lambda o: o.route(Tensor((3, 2), "int64"), 4, I((3, 2)), I((5,))),
+    "route slots of another shape": lambda o: o.route(I((3, 2)), 4, I((2, 3)), I((5,))),
+    "route too few offsets": lambda o: o.route(I((3, 2)), 4, I((3, 2)), I((4,))),
+    "route order of another length": lambda o: o.route(I((3, 2)), 4, I((3, 2)), I((5,)), order=I((5,))),
+    "route choices with gaps": lambda o: o.route(I((3, 2), stride=(4, 1)), 4, I((3, 2)), I((5,))),
+    "dispatch with other rows": lambda o: o.dispatch(T((3, 4)), I((2, 2)), T((6, 4))),
+    "dispatch with other columns": lambda o: o.dispatch(T((3, 4)), I((3, 2)), T((6, 5))),
+    "dispatch to another type": lambda o: o.dispatch(T((3, 4)), I((3, 2)), T((6, 4), "float16")),
+    "dispatch with a vector of slots": lambda o: o.dispatch(T((3, 4)), I((3,)), T((6, 4))),
+    "combine to another shape": lambda o: o.combine(T((6, 4)), I((3, 2)), T((6, 4))),
+    "combine weights of another shape": lambda o: o.combine(T((6, 4)), I((3, 2)), T((3, 4)), weights=T((2, 3))),
+    "combine weights of integers": lambda o: o.combine(T((6, 4)), I((3, 2)), T((3, 4)), weights=I((3, 2))),
+    "combine gradient without rows": lambda o: o.combine_grad(T((3, 4)), None, I((3, 2)), T((3, 2)), T((6, 4)), T((3, 2))),
+    "combine gradient of other rows": lambda o: o.combine_grad(T((3, 4)), T((6, 4)), I((3, 2)), T((3, 2)), T((5, 4)), T((3, 2))),
+    "combine gradient of another weight type": lambda o: o.combine_grad(T((3, 4)), T((6, 4)), I((3, 2)), T((3, 2)), T((6, 4)),
+                                                                      T((3, 2), "bfloat16")),
+    "quantize to unsigned bytes": lambda o: o.quantize(T((3, 4)), Tensor((3, 4), "uint8"), T((3,))),
+    "quantize to another shape": lambda o: o.quantize(T((3, 4)), q8((3, 5)), T((3,))),
+    "quantize scales by column": lambda o: o.quantize(T((3, 4)), q8((3, 4)), T((4,))),
+    "product of float rows": lambda o: o.product(T((3, 8)), T((3,)), q8((5, 8)), T((5,)), T((3, 5))),
+    "product of other lengths": lambda o: o.product(q8((3, 8)), T((3,)), q8((5, 9)), T((5,)), T((3, 5))),
+    "product with scales by k": lambda o: o.product(q8((3, 8)), T((8,)), q8((5, 8)), T((5,)), T((3, 5))),
+    "product to integers": lambda o: o.product(q8((3, 8)), T((3,)), q8((5, 8)), T((5,)), I((3, 5))),
+    "product groups without a dimension": lambda o: o.product(q8((3, 8)), T((3,)), q8((5, 8)), T((5,)), T((3, 5)), offsets=I((2,))),
+    "product groups of other offsets": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8)), T((2, 5)), T((3, 5)), offsets=I((2,))),
+    "product groups that overlap": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8), stride=(8, 8, 1)), T((2, 5)), T((3, 5)),
+                                                       offsets=I((3,))),
+    "product with a bias for all groups": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8)), T((2, 5)), T((3, 5)), bias=T((5,)),
+                                                              offsets=I((3,))),
+}
+
+
+@pytest.mark.parametrize("what", sorted(BAD))
+def test_refused(ops, what):
+    with pytest.raises((ValueError, TypeError)):
+        BAD[what](ops)
+    assert ops.ctx.lib.calls == []
+
+
+def test_arguments_reach_the_library_in_the_header_s_order(ops):
+    ops.lookup(T((9, 4), stride=(6, 1), at=0x10), Tensor((3,), "int64", at=0x20), T((3, 4), stride=(5, 1), at=0x30), scale=2.0)
+    ops.product(q8((3, 8), at=0x10), T((3,), at=0x20), q8((2, 5, 8), stride=(60, 10, 1), at=0x30), T((2, 5), at=0x40),
+                Tensor((3, 5), "float16", at=0x50), bias=T((2, 5), at=0x60), offsets=I((3,), at=0x70))
+    ops.combine_grad(T((3, 4), at=0x10), T((6, 4), at=0x20), I((3, 2), at=0x30), T((3, 2), at=0x40), T((6, 4), at=0x50), None)
+    assert ops.ctx.lib.calls == [
+        ("skm_lookup_rows", (1, 0x10, 0, 9, 4, 6, 0x20, 4, 3, 2.0, 0x30, 5)),
+        ("skm_product_i8", (1, 0x10, 3, 8, 0x20, 0x30, 5, 8, 10, 0x40, 0x60, 2, 60, 0x70, 0x50, 1, 5)),
+        ("skm_combine_rows_grad", (1, 0x10, 0, 3, 4, 4, 0x20, 6, 4, 0x30, 2, 0x40, 0, 0x50, 4, None)),
+    ]
+
+
+def test_one_row_may_have_any_stride(ops):
+    """A library may give a tensor of one row any row stride, and one of a single column any column stride."""
+    ops.lookup(T((9, 4)), I((1,)), T((1, 4), stride=(0, 1)))
+    ops.dispatch(T((3, 1), stride=(1, 7)), I((3, 2)), T((6, 1), stride=(1, 3)))
+    assert len(ops.ctx.lib.calls) == 2
+
+
+def test_scratch_sizes_need_no_device(capi):
+    import ctypes
+
+    lib = capi.load()
+    need = ctypes.c_size_t()
+    assert lib.skm_route_scratch(0, 2, 8, ctypes.byref(need)) == 0 and need.value == 0
+    assert lib.skm_route_scratch(64, 8, 64, ctypes.byref(need)) == 0 and need.value == 0  # one launch, no scratch
+    sizes = []
+    for n in (10000, 100000, 1000000):
+        assert lib.skm_route_scratch(n, 2, 64, ctypes.byref(need)) == 0
+        sizes.append(need.value)
+    assert 0 < sizes[0] < sizes[1] < sizes[2] < 64 << 20
+    assert lib.skm_route_scratch(1 << 20, 1 << 11, 8, ctypes.byref(need)) == capi.SKM_ERR_INVALID
+    assert lib.skm_route_scratch(4, 2, 0, ctypes.byref(need)) == capi.SKM_ERR_INVALID
+    assert lib.skm_lookup_rows_grad_scratch(100000, 65536, 64, ctypes.byref(need)) == 0 and need.value > 100000 * 4
+    assert lib.skm_lookup_rows_grad_scratch(10, 10, 0, ctypes.byref(need)) == capi.SKM_ERR_INVALID
+
+
+def test_null_context_is_refused(capi):
+    lib = capi.load()
+    assert lib.skm_lookup_rows(None, None, 0, 1, 1, 1, None, 3, 1, 1.0, None, 1) == capi.SKM_ERR_INVALID
+    assert lib.skm_route(None, None, 1, 1, 1, None, None, None, None, 0) == capi.SKM_ERR_INVALID
+    assert lib.skm_product_i8(None, None, 1, 1, None, None, 1, 1, 1, None, None, 0, 0, None, None, 0, 1) == capi.SKM_ERR_INVALID
+    assert lib.skm_quantize_rows(None, None, 0, 1, 1, 1, None, 1, None) == capi.SKM_ERR_INVALID
