@@ -120,88 +120,335 @@ __device__ __forceinline__ RowTile find_rows(const ProductArgs& p, const uint32_
     return {0, 0, 0};
 }
 
-// 16 columns of a row from column k on, zeros past the last one.  W: the bytes that pointers and strides are aligned to.
-template <int W>
-__device__ __forceinline__ intx4 load_columns(const int8_t* row, const uint32_t k, const uint32_t columns) {
-    if constexpr (W == 16) {
-        if (k + 16 <= columns) return *reinterpret_cast<const intx4*>(row + k);
+// 16 bytes of a row.  Rows that are not aligned to 16 bytes are read with the same instruction, which takes any address;
+// only the compiler has to be told.
+template <bool ALIGNED>
+__device__ __forceinline__ intx4 load16(const int8_t* p) {
+    if constexpr (ALIGNED) return *reinterpret_cast<const intx4*>(p);
+    intx4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+// The 16 bytes from column k on of a row of `columns` >= 16, zeros past its end: where fewer are left, the last 16 of the row,
+// shifted.
+__device__ __forceinline__ intx4 load16_end(const int8_t* row, const int k, const int columns) {
+    const int left = columns - k;
+    const int8_t* from = row + (left >= 16 ? k : columns - 16);
+    unsigned long long half[2];
+    __builtin_memcpy(half, from, 16);
+    int drop = left >= 16 ? 0 : 16 - left;  // bytes that are before column k
+    if (drop >= 8) {
+        half[0] = half[1];
+        half[1] = 0;
+        drop -= 8;
     }
-    intx4 v = {};
-    if constexpr (W >= 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (k + 4 * i + 4 <= columns) v[i] = *reinterpret_cast<const int*>(row + k + 4 * i);
-            else
-                for (uint32_t j = 0; j < 4; ++j)
-                    if (k + 4 * i + j < columns) v[i] |= (int) (uint8_t) row[k + 4 * i + j] << (8 * j);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-                if (k + 4 * i + j < columns) v[i] |= (int) (uint8_t) row[k + 4 * i + j] << (8 * j);
-    }
+    drop = min(drop, 7);
+    half[0] = half[0] >> (8 * drop) | (half[1] << 1) << (63 - 8 * drop);
+    half[1] >>= 8 * drop;
+    if (left <= 0) half[0] = half[1] = 0;
+    intx4 v;
+    __builtin_memcpy(&v, half, 16);
+    return v;
+}
+// The same for a row of any length.
+__device__ __forceinline__ intx4 load16_short(const int8_t* row, const int k, const int columns) {
+    unsigned long long half[2] = {0, 0};
+#pragma unroll 1
+    for (int i = 0; i < 16 && k + i < columns; ++i) half[i >> 3] |= (unsigned long long) (uint8_t) row[k + i] << (8 * (i & 7));
+    intx4 v;
+    __builtin_memcpy(&v, half, 16);
     return v;
 }
 
-template <class O>
-__device__ __forceinline__ void put(void* out, const size_t at, const float v) {
-    reinterpret_cast<O*>(out)[at] = (O) v;
+// ---- few rows: the weights go from memory to the registers, once ----
+//
+// A workgroup owns 16 RT rows and 16 NB columns of the result; its wavefronts share the columns of the operands, and
+// their 32-bit sums are added through LDS (exact, so the split does not show).  With a row or a few per matrix every
+// byte of the weights is read once and used at once, so nothing is gained by LDS; what counts is how many bytes are on their
+// way: each wavefront requests AHEAD steps of 64 columns before it uses the first.
+template <class O, int RT, int NB, int WAVES, int AHEAD, bool ALIGNED>
+__global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs p, const uint32_t tiles_n) {
+    constexpr int TM = 16 * RT, TN = 16 * NB;
+    __shared__ int part[WAVES][TM][TN + 4];
+    const RowTile rows = find_rows(p, TM, blockIdx.x / tiles_n);
+    if (rows.first >= rows.end) return;
+    const uint32_t n0 = blockIdx.x % tiles_n * TN;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // lane l holds row l % 16 of a block and 16 columns from 16 (l / 16) on
+    const int8_t *a[RT], *b[NB];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) a[i] = p.a + (size_t) min(rows.first + i * 16 + (lane & 15), rows.end - 1) * p.a_stride + (lane >> 4) * 16;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+        b[j] = p.b + rows.group * p.b_group_stride + (size_t) min(n0 + j * 16 + (lane & 15), p.n - 1) * p.b_stride + (lane >> 4) * 16;
+    intx4 acc[NB][RT] = {};
+    const uint32_t steps = (p.k + 63) / 64, each = (steps + WAVES - 1) / WAVES;
+    const uint32_t from = min(wave * each, steps), to = min(from + each, steps), full = min(to, p.k / 64);
+    const auto multiply = [&](const intx4 (&x)[RT], const intx4 (&w)[NB]) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[j][i], 0, 0, 0);
+    };
+    uint32_t s = from;
+    if (s + AHEAD <= full) {
+        intx4 x[AHEAD][RT], w[AHEAD][NB];
+        const auto request = [&](const int q, const uint32_t step) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) w[q][j] = load16<ALIGNED>(b[j] + (size_t) step * 64);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) x[q][i] = load16<ALIGNED>(a[i] + (size_t) step * 64);
+        };
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) request(q, s + q);
+        for (; s + 2 * AHEAD <= full; s += AHEAD)
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                multiply(x[q], w[q]);
+                request(q, s + AHEAD + q);
+            }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) multiply(x[q], w[q]);
+        s += AHEAD;
+    }
+    for (; s < to; ++s) {
+        intx4 x[RT], w[NB];
+        const int skip = (lane >> 4) * 16, k = (int) (s * 64) + skip;
+        if (p.k >= 16) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) w[j] = load16_end(b[j] - skip, k, (int) p.k);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) x[i] = load16_end(a[i] - skip, k, (int) p.k);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) w[j] = load16_short(b[j] - skip, k, (int) p.k);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) x[i] = load16_short(a[i] - skip, k, (int) p.k);
+        }
+        multiply(x, w);
+    }
+    // block (j, i): lane l holds the columns 4 (l / 16) .. + 3 of the result's row l % 16
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+            *reinterpret_cast<intx4*>(&part[wave][i * 16 + (lane & 15)][j * 16 + (lane >> 4) * 4]) = acc[j][i];
+    __syncthreads();
+    const float* b_scale = p.b_scale + (size_t) rows.group * p.n;
+    const float* bias = p.bias ? p.bias + (size_t) rows.group * p.n : nullptr;
+    for (uint32_t e = threadIdx.x; e < TM * TN; e += WAVES * 64) {
+        const uint32_t r = e / TN, c = e % TN, m = rows.first + r, n = n0 + c;
+        if (m >= rows.end || n >= p.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) sum += part[v][r][c];
+        const float value = (float) sum * p.a_scale[m] * b_scale[n] + (bias ? bias[n] : 0.0f);
+        reinterpret_cast<O*>(p.out)[(size_t) m * p.out_stride + n] = (O) value;
+    }
 }
 
-// 128 x 128 tiles, four wavefronts of 64 x 64 in 32 x 32 blocks, 64 columns of both operands at a time in LDS.
-constexpr int TILE = 128, TILE_K = 64, TILE_STRIDE = TILE_K + 16;  // 16 bytes of padding: rows start in different banks
+// ---- many rows: tiles through LDS ----
+//
+// Four wavefronts, each FM x FN blocks of 32 x 32, so a tile is 64 FM x 64 FN.  A stage is 128 columns (a cache line) of
+// both operands; two stages are in LDS and a third is on its way in registers.  A wavefront reads (FM + FN) KB of LDS for each
+// FM FN instructions: at 4 x 4 half of what the LDS can give in the time of the matrix instructions, at 2 x 4 (eight
+// wavefronts for the same tile) three quarters, and the stages' stores come on top.
+// Chunks of 16 bytes are stored at position chunk ^ (row % 8) of their row, so that the 32 rows of a block, 128 bytes
+// apart, are read from different banks.
+constexpr int STAGE_K = 128;
 
-template <class O, int W>
-__global__ __launch_bounds__(256) void product_tile_kernel(const ProductArgs p, const uint32_t tiles_n) {
-    __shared__ __align__(16) int8_t As[TILE * TILE_STRIDE];
-    __shared__ __align__(16) int8_t Bs[TILE * TILE_STRIDE];
-    const RowTile rows = find_rows(p, TILE, blockIdx.x / tiles_n);
+template <int FM, int FN>
+constexpr size_t tiles_lds_bytes() {
+    return (size_t) 2 * (64 * FM + 64 * FN) * STAGE_K;
+}
+
+// Number of a workgroup to tile: workgroups whose number is equal mod 8 run on the same die and share its L2, where 32 of them
+// at a time take a block of `super_m` x 32 / super_m neighbouring tiles.
+struct TileMap {
+    uint32_t super_m, super_n, across, tiles_n;
+    __device__ __forceinline__ bool operator()(const uint32_t number, uint32_t& tile_m, uint32_t& tile_n) const {
+        const uint32_t die = number & 7, local = number >> 3;
+        const uint32_t super = (local >> 5) * 8 + die, within = local & 31;
+        tile_m = super / across * super_m + within % super_m;
+        tile_n = super % across * super_n + within / super_m;
+        return tile_n < tiles_n;
+    }
+};
+
+template <class O, int FM, int FN, bool ALIGNED>
+__global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(const ProductArgs p, const TileMap map) {
+    constexpr int TM = 64 * FM, TN = 64 * FN, NLA = TM / 32, NLB = TN / 32;
+    constexpr uint32_t STAGE = (TM + TN) * STAGE_K;
+    extern __shared__ __align__(16) int8_t lds[];  // [2][TM + TN][STAGE_K]
+    uint32_t tile_m, tile_n;
+    if (!map(blockIdx.x, tile_m, tile_n)) return;
+    const RowTile rows = find_rows(p, TM, tile_m);
     if (rows.first >= rows.end) return;
-    const uint32_t n0 = blockIdx.x % tiles_n * TILE;
+    const uint32_t n0 = tile_n * TN;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    const int8_t* b = p.b + (size_t) rows.group * p.b_group_stride;
-    intx16 acc[2][2] = {};
-    for (uint32_t k0 = 0; k0 < p.k; k0 += TILE_K) {
+    const uint32_t wm = (wave >> 1) * FM * 32, wn = (wave & 1) * FN * 32;
+
+    // memory to registers: a thread takes 16 bytes of every 32nd row; rows past the end repeat the last one and are not stored
+    const uint32_t ld_row = tid >> 3, ld_chunk = tid & 7;
+    const int8_t* a_base = p.a + (size_t) rows.first * p.a_stride;
+    const int8_t* b_base = p.b + rows.group * p.b_group_stride + (size_t) n0 * p.b_stride;
+    uint32_t a_at[NLA], b_at[NLB];
+#pragma unroll
+    for (int i = 0; i < NLA; ++i) a_at[i] = min(ld_row + 32 * i, rows.end - 1 - rows.first) * (uint32_t) p.a_stride + ld_chunk * 16;
+#pragma unroll
+    for (int i = 0; i < NLB; ++i) b_at[i] = min(ld_row + 32 * i, p.n - 1 - n0) * (uint32_t) p.b_stride + ld_chunk * 16;
+    intx4 ra[NLA], rb[NLB];
+    const uint32_t stages = (p.k + STAGE_K - 1) / STAGE_K, full = p.k / STAGE_K;
+    const auto request = [&](const uint32_t s) {
+        const int8_t *as = a_base + (size_t) s * STAGE_K, *bs = b_base + (size_t) s * STAGE_K;
+#pragma unroll
+        for (int i = 0; i < NLA; ++i) ra[i] = load16<ALIGNED>(as + a_at[i]);
+#pragma unroll
+        for (int i = 0; i < NLB; ++i) rb[i] = load16<ALIGNED>(bs + b_at[i]);
+    };
+    const auto request_last = [&](const uint32_t s) {  // a stage that the rows end in
+        const int k = (int) (s * STAGE_K + ld_chunk * 16);
+#pragma unroll
+        for (int i = 0; i < NLA; ++i) ra[i] = load16_end(a_base + (a_at[i] - ld_chunk * 16), k, (int) p.k);
+#pragma unroll
+        for (int i = 0; i < NLB; ++i) rb[i] = load16_end(b_base + (b_at[i] - ld_chunk * 16), k, (int) p.k);
+    };
+    const auto request_any = [&](const uint32_t s) {
+        if (s < full) request(s);
+        else request_last(s);
+    };
+    const uint32_t st = ld_row * STAGE_K + ((ld_chunk ^ (ld_row & 7)) << 4);
+    const auto publish = [&](const uint32_t buffer) {
+        int8_t* to = lds + buffer * STAGE + st;
+#pragma unroll
+        for (int i = 0; i < NLA; ++i) *reinterpret_cast<intx4*>(to + i * 32 * STAGE_K) = ra[i];
+#pragma unroll
+        for (int i = 0; i < NLB; ++i) *reinterpret_cast<intx4*>(to + (TM + i * 32) * STAGE_K) = rb[i];
+    };
+    // registers of a block: lane l holds row l % 32 and 16 columns from 16 (l / 32) on
+    const uint32_t fr = (lane & 31) * STAGE_K;
+    intx4 fa[2][FM], fb[2][FN];
+    const auto fetch = [&](const uint32_t buffer, const int slice, const int to) {
+        const int8_t* at = lds + buffer * STAGE + fr + (((2 * slice + (lane >> 5)) ^ (lane & 7)) << 4);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const intx4*>(at + (wm + i * 32) * STAGE_K);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[to][j] = *reinterpret_cast<const intx4*>(at + (TM + wn + j * 32) * STAGE_K);
+    };
+    intx16 acc[FM][FN] = {};
+    const auto multiply = [&](const int of) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[of][j], fa[of][i], acc[i][j], 0, 0, 0);
+    };
+
+    // One stage: its slices 1 to 3 are read while the slices before them are multiplied; the barrier sits before the last
+    // slice's products, when every read of the stage has returned, and the next stage's first slice is read under them.
+    const auto stage = [&](const uint32_t s, auto hot) {  // hot: stages s + 1 and s + 2 exist and are whole
+        constexpr bool HOT = decltype(hot)::value;
+        const uint32_t cur = s & 1;
+        if (HOT || s + 1 < stages) publish(cur ^ 1);  // its last readers passed the barrier of stage s - 1
+        if (HOT) request(s + 2);
+        else if (s + 2 < stages) request_any(s + 2);
+        fetch(cur, 1, 1);
+        multiply(0);
+        fetch(cur, 2, 0);
+        multiply(1);
+        fetch(cur, 3, 1);
+        multiply(0);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t r = (tid >> 2) + i * 64, c = (tid & 3) * 16;
-            const uint32_t row_a = min(rows.first + r, rows.end - 1), row_b = min(n0 + r, p.n - 1);  // repeated rows are not stored
-            *reinterpret_cast<intx4*>(&As[r * TILE_STRIDE + c]) = load_columns<W>(p.a + (size_t) row_a * p.a_stride, k0 + c, p.k);
-            *reinterpret_cast<intx4*>(&Bs[r * TILE_STRIDE + c]) = load_columns<W>(b + (size_t) row_b * p.b_stride, k0 + c, p.k);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < TILE_K; kk += 32) {
-            intx4 fa[2], fb[2];
-            const uint32_t c = kk + (lane >> 5) * 16;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = *reinterpret_cast<const intx4*>(&As[(wm + i * 32 + (lane & 31)) * TILE_STRIDE + c]);
-                fb[i] = *reinterpret_cast<const intx4*>(&Bs[(wn + i * 32 + (lane & 31)) * TILE_STRIDE + c]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
-        }
+        if (HOT || s + 1 < stages) fetch(cur ^ 1, 0, 0);
+        multiply(1);
+    };
+    request_any(0);
+    publish(0);
+    if (stages > 1) request_any(1);
+    __syncthreads();
+    fetch(0, 0, 0);
+    uint32_t s = 0;
+    for (; s + 2 < full; ++s) stage(s, std::true_type{});
+#pragma unroll 1
+    for (; s < stages; ++s) stage(s, std::false_type{});
+
+    // Results, 32 rows at a time through LDS (each wavefront in a part of its own), so that rows are stored 16 bytes per lane.
+    // Element r of block (i, j): row l % 32, column 8 (r / 4) + 4 (l / 32) + r % 4.
+    constexpr int E = 16 / sizeof(O), COLUMNS = FN * 32, LD = COLUMNS + E;
+    static_assert((size_t) 4 * 32 * LD * sizeof(O) + 2 * TN * sizeof(float) <= (size_t) 2 * STAGE, "results go through the stages' LDS");
+    __syncthreads();
+    O* staged = reinterpret_cast<O*>(lds) + wave * 32 * LD;
+    float* b_scale = reinterpret_cast<float*>(lds + (size_t) 4 * 32 * LD * sizeof(O));
+    float* bias = b_scale + TN;
+    if (tid < TN) {
+        const size_t n = (size_t) rows.group * p.n + min(n0 + tid, p.n - 1);
+        b_scale[tid] = p.b_scale[n];
+        bias[tid] = p.bias ? p.bias[n] : 0.0f;
     }
+    __syncthreads();
+    O* out = reinterpret_cast<O*>(p.out);
+    const bool wide = ((reinterpret_cast<size_t>(out) | p.out_stride * sizeof(O)) & 15) == 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t n = n0 + wn + j * 32 + (lane & 31);
-        if (n >= p.n) continue;
-        const float b_scale = p.b_scale[(size_t) rows.group * p.n + n];
-        const float bias = p.bias ? p.bias[(size_t) rows.group * p.n + n] : 0.0f;
+    for (int i = 0; i < FM; ++i) {
+        const uint32_t m0 = rows.first + wm + i * 32;
+        const float a_scale = p.a_scale[min(m0 + (lane & 31), rows.end - 1)];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const uint32_t m = rows.first + wm + i * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                if (m < rows.end) put<O>(p.out, (size_t) m * p.out_stride + n, (float) acc[i][j][r] * p.a_scale[m] * b_scale + bias);
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t c = j * 32 + 8 * r + 4 * (lane >> 5);
+                const vec_of<float, 4> scale = *reinterpret_cast<const vec_of<float, 4>*>(&b_scale[wn + c]);
+                const vec_of<float, 4> shift = *reinterpret_cast<const vec_of<float, 4>*>(&bias[wn + c]);
+                vec_of<float, 4> v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] = (float) acc[i][j][4 * r + q] * a_scale * scale[q] + shift[q];
+                *reinterpret_cast<vec_of<O, 4>*>(&staged[(lane & 31) * LD + c]) = narrow<O, 4>(v);
             }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int q = 0; q < 32 * COLUMNS / (64 * E); ++q) {
+            const uint32_t r = (q * 64 + lane) / (COLUMNS / E), c = (q * 64 + lane) % (COLUMNS / E) * E;
+            const uint32_t m = m0 + r, n = n0 + wn + c;
+            if (m >= rows.end || n >= p.n) continue;
+            const vec_of<O, E> v = *reinterpret_cast<const vec_of<O, E>*>(&staged[r * LD + c]);
+            O* to = out + (size_t) m * p.out_stride + n;
+            if (wide && n + E <= p.n) *reinterpret_cast<vec_of<O, E>*>(to) = v;
+            else
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (n + e < p.n) to[e] = v[e];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+}
+
+template <class O, int RT, int NB, int WAVES, int AHEAD>
+int launch_few_rows(skm_ctx* ctx, const ProductArgs& p, const bool aligned) {
+    const uint32_t tiles_n = (p.n + 16 * NB - 1) / (16 * NB);
+    const uint64_t blocks = ((uint64_t) (p.m + 16 * RT - 1) / (16 * RT) + (p.offsets ? p.groups : 0)) * tiles_n;
+    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
+    if (aligned) product_few_rows_kernel<O, RT, NB, WAVES, AHEAD, true><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
+    else product_few_rows_kernel<O, RT, NB, WAVES, AHEAD, false><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
+    return check_hip(hipGetLastError(), "product_few_rows_kernel launch");
+}
+
+template <class O, int FM, int FN>
+int launch_tiles(skm_ctx* ctx, const ProductArgs& p, const bool aligned) {
+    constexpr size_t lds = tiles_lds_bytes<FM, FN>();
+    const uint32_t tiles_n = (p.n + 64 * FN - 1) / (64 * FN);
+    const uint64_t tiles_m = (uint64_t) (p.m + 64 * FM - 1) / (64 * FM) + (p.offsets ? p.groups : 0);
+    uint32_t super_n = 1;
+    while (super_n < 8 && super_n < tiles_n) super_n *= 2;
+    const uint32_t super_m = 32 / super_n, across = (tiles_n + super_n - 1) / super_n;
+    const uint64_t supers = (tiles_m + super_m - 1) / super_m * across, blocks = (supers + 7) / 8 * 8 * 32;
+    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
+    const TileMap map{super_m, super_n, across, tiles_n};
+    const auto launch = [&](auto kernel) {
+        SKM_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds),
+                          "hipFuncSetAttribute(MaxDynamicSharedMemorySize)"));
+        kernel<<<(unsigned) blocks, 256, lds, ctx->stream>>>(p, map);
+        return check_hip(hipGetLastError(), "product_tiles_kernel launch");
+    };
+    return aligned ? launch(product_tiles_kernel<O, FM, FN, true>) : launch(product_tiles_kernel<O, FM, FN, false>);
 }
 
 } // namespace
@@ -264,17 +511,18 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
     ScopedStage st(ctx, "rows/product");
     const ProductArgs p{d_a, d_a_scale, d_b, d_b_scale, d_bias, d_offsets, d_out, a_stride, b_stride, d_offsets ? b_group_stride : 0,
                         out_stride, (uint32_t) m, (uint32_t) n, (uint32_t) k, d_offsets ? (uint32_t) groups : 1};
-    const size_t width = common_width({address(d_a), address(d_b), a_stride, b_stride, p.b_group_stride});
+    const bool aligned = common_width({address(d_a), address(d_b), a_stride, b_stride, p.b_group_stride}) == 16;
     return for_type(out_type, [&](auto sample) {
         using O = decltype(sample);
-        const uint32_t tiles_n = (uint32_t) ((n + TILE - 1) / TILE);
-        const uint64_t tiles_m = (m + TILE - 1) / TILE + (d_offsets ? groups : 0);
-        SKM_REQUIRE(tiles_m * tiles_n <= 0x7fffffffULL, "too many tiles for one launch");
-        const unsigned blocks = (unsigned) (tiles_m * tiles_n);
-        if (width == 16) product_tile_kernel<O, 16><<<blocks, 256, 0, ctx->stream>>>(p, tiles_n);
-        else if (width >= 4) product_tile_kernel<O, 4><<<blocks, 256, 0, ctx->stream>>>(p, tiles_n);
-        else product_tile_kernel<O, 1><<<blocks, 256, 0, ctx->stream>>>(p, tiles_n);
-        return check_hip(hipGetLastError(), "product_tile_kernel launch");
+        const size_t rows = d_offsets ? (m + groups - 1) / groups : m;  // of a group, on average
+        const bool near = k >= 16 && a_stride < (1u << 23) && b_stride < (1u << 23);  // as the tiles' loads assume (32-bit offsets)
+        const uint64_t parts = d_offsets ? groups : 1;
+        const uint64_t large = parts * ((rows + 255) / 256) * ((n + 255) / 256), medium = parts * ((rows + 127) / 128) * ((n + 127) / 128);
+        if (near && rows > 128 && large >= 192) return launch_tiles<O, 4, 4>(ctx, p, aligned);
+        if (near && rows > 64 && medium >= 128) return launch_tiles<O, 2, 2>(ctx, p, aligned);
+        if (rows > 16) return launch_few_rows<O, 4, 2, 8, 2>(ctx, p, aligned);
+        if (rows > 4) return launch_few_rows<O, 2, 2, 8, 4>(ctx, p, aligned);
+        return launch_few_rows<O, 1, 2, 8, 4>(ctx, p, aligned);
     });
 }
 
