@@ -231,6 +231,17 @@ class DeviceArray:
         check(self.ctx.lib.skm_download(self.ctx.handle, out.ctypes.data, self.ptr, out.nbytes))
         return out
 
+    def stride(self):
+        """Elements between neighbours of each dimension."""
+        steps, step = [], 1
+        for size in reversed(self.shape):
+            steps.insert(0, step)
+            step *= size
+        return tuple(steps)
+
+    def data_ptr(self):
+        return self.ptr
+
     def offset(self, elements):
         """Device address `elements` items past the start."""
         return self.ptr + int(elements) * self.dtype.itemsize

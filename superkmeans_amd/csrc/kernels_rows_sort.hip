@@ -5,18 +5,23 @@
 // choices before it in the order (group, place), and a table row's gradient adds its tokens in that order.  There are
 // no floating-point atomics.
 //
-// One pass of the sort over `bins` digit values is three launches.  A wavefront owns a tile of consecutive elements and
-// walks it 64 at a time: lanes with equal digits find each other with one ballot per digit bit, a counter per digit in LDS
-// carries the tile's count from round to round, and every element's rank in its tile is stored.  Then one wavefront per
-// digit scans its row of tile counts, and the last launch adds the three numbers that make up an element's place.
-// Against a sort by 8-bit digits this needs one pass for up to 2,048 groups and two for tables of up to 4 million rows.
+// One pass of the sort over `bins` digit values is two launches.  A workgroup of 16 wavefronts owns a tile of consecutive
+// elements and every wavefront a contiguous share of it, which it walks 64 at a time: lanes with equal digits find each other
+// with one ballot per digit bit, and a counter per digit and wavefront in LDS carries the count from round to round.  That
+// gives every element's rank in its tile, and the tile its counts.  The second launch adds up the counts of the tiles
+// before (every workgroup reads the whole table, which is small; with many tiles a launch in between scans it) and moves
+// the elements.  Up to 8,192 choices are one tile, and one launch.  With 10-bit digits a route takes one pass for up to 1,023
+// groups and a table of up to a million rows two.
 #include "rows_common.h"
 
 namespace skm {
 namespace {
 
-constexpr int MAX_DIGIT_BITS = 11;
-constexpr uint32_t MAX_BINS = 1u << MAX_DIGIT_BITS;
+constexpr int MAX_DIGIT_BITS = 10;
+constexpr uint32_t MAX_BINS = 1u << MAX_DIGIT_BITS;  // a thread of a workgroup each
+constexpr int SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / 64;
+constexpr int MAX_ROUNDS = 8;
+constexpr uint32_t TILES_WITHOUT_SCAN = 128;
 
 // Where an element's key comes from: table ids or choices as the caller has them (anything outside [0, limit) becomes
 // limit), or the keys that the pass before left.
@@ -50,107 +55,154 @@ __device__ __forceinline__ uint32_t wave_inclusive_sum(uint32_t v, const uint32_
     return v;
 }
 
-// First launch of a pass, one wavefront per tile.
-__global__ __launch_bounds__(64) void tile_ranks_kernel(
-    const KeySource source, const size_t n, const int shift, const uint32_t mask, const int bits, const uint32_t bins,
-    const uint32_t rounds, const uint32_t n_tiles, uint16_t* __restrict__ ranks, uint32_t* __restrict__ counts
-) {
-    extern __shared__ uint32_t count[];
-    const uint32_t lane = threadIdx.x;
-    for (uint32_t b = lane; b < bins; b += 64) count[b] = 0;
+// Exclusive sum over the threads of a workgroup; ends on a barrier.
+__device__ __forceinline__ uint32_t block_exclusive_sum(const uint32_t v, uint32_t* wave_sum) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t incl = wave_inclusive_sum(v, lane);
+    if (lane == 63) wave_sum[wave] = incl;
     __syncthreads();
-    const size_t first = (size_t) blockIdx.x * rounds * 64;
-    for (uint32_t r = 0; r < rounds; ++r) {
-        const size_t i = first + (size_t) r * 64 + lane;
-        const bool in = i < n;
-        const uint32_t digit = in ? (source(i) >> shift) & mask : 0;
-        const unsigned long long match = equal_lanes(in, digit, bits);
-        const uint32_t below = (uint32_t) __popcll(match & lanes_below(lane));
-        const uint32_t before = in ? count[digit] : 0;
-        __syncthreads();  // one wavefront: orders the reads before the writes
-        if (in) {
-            ranks[i] = (uint16_t) (before + below);
-            if (below == 0) count[digit] = before + (uint32_t) __popcll(match);
-        }
-        __syncthreads();
-    }
-    for (uint32_t b = lane; b < bins; b += 64) counts[(size_t) b * n_tiles + blockIdx.x] = count[b];
+    uint32_t base = incl - v;
+    for (uint32_t w = 0; w < wave; ++w) base += wave_sum[w];
+    __syncthreads();
+    return base;
 }
 
-// Second launch: one wavefront per digit turns its row of tile counts into the counts of the tiles before, and leaves the
-// digit's total.
+// Where a pass puts its elements: a radix pass their keys and indices, the only pass of a route the slots, the order
+// and the offsets (bin `bins - 1` then holds the dropped choices).
+struct Places {
+    const uint32_t* index_in;  // null: an element's index is its position
+    uint32_t *keys, *index;
+    uint32_t *slots, *order, *offsets;
+    template <bool ROUTE>
+    __device__ __forceinline__ void put(const size_t i, const uint32_t key, const uint32_t limit, const uint32_t place) const {
+        if (ROUTE) {
+            const bool kept = key < limit;
+            slots[i] = kept ? place : SKM_NO_ROW;
+            if (order) order[place] = kept ? (uint32_t) i : SKM_NO_ROW;
+        } else {
+            keys[place] = key;
+            index[place] = index_in ? index_in[i] : (uint32_t) i;
+        }
+    }
+};
+
+// First launch of a pass: ranks in the tile and the tile's counts.  ONLY: the tile is all there is, and a route is done
+// with it.
+template <int ROUNDS, bool ONLY>
+__global__ __launch_bounds__(SORT_THREADS) void tile_ranks_kernel(
+    const KeySource source, const size_t n, const int shift, const uint32_t mask, const int bits, const uint32_t bins,
+    uint16_t* __restrict__ ranks, uint32_t* __restrict__ counts, const Places places
+) {
+    extern __shared__ uint16_t count[];  // [SORT_WAVES][bins]; a tile has at most 8,192 elements
+    __shared__ uint32_t wave_sum[SORT_WAVES];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (uint32_t b = tid; b < SORT_WAVES * bins; b += SORT_THREADS) count[b] = 0;
+    const size_t first = (size_t) blockIdx.x * (SORT_THREADS * ROUNDS) + wave * (ROUNDS * 64) + lane;
+    uint32_t key[ROUNDS], rank[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) key[r] = first + r * 64 < n ? source(first + r * 64) : 0;
+    __syncthreads();
+    uint16_t* mine = count + wave * bins;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const bool in = first + r * 64 < n;
+        const uint32_t digit = (key[r] >> shift) & mask;
+        const unsigned long long match = equal_lanes(in, digit, bits);
+        const uint32_t below = (uint32_t) __popcll(match & lanes_below(lane));
+        const uint32_t before = in ? mine[digit] : 0;
+        rank[r] = before + below;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wavefront's LDS accesses stay in this order
+        if (in && below == 0) mine[digit] = (uint16_t) (before + __popcll(match));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    // thread b: the counts of digit b in the wavefronts before
+    uint32_t total = 0;
+    if (tid < bins)
+        for (int w = 0; w < SORT_WAVES; ++w) {
+            const uint32_t c = count[w * bins + tid];
+            count[w * bins + tid] = (uint16_t) total;
+            total += c;
+        }
+    if (ONLY) {
+        const uint32_t base = block_exclusive_sum(total, wave_sum);
+        if (tid < bins) {
+            places.offsets[tid] = base;
+            for (int w = 0; w < SORT_WAVES; ++w) count[w * bins + tid] += (uint16_t) base;
+        }
+    } else if (tid < bins) {
+        counts[(size_t) blockIdx.x * bins + tid] = total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const size_t i = first + r * 64;
+        if (i >= n) continue;
+        const uint32_t at = mine[(key[r] >> shift) & mask] + rank[r];
+        if (ONLY) places.put<true>(i, key[r], source.limit, at);
+        else ranks[i] = (uint16_t) at;
+    }
+}
+
+// With many tiles: a wavefront per digit turns the tiles' counts into the counts of the tiles before, and leaves the total.
 __global__ __launch_bounds__(64) void tile_counts_scan_kernel(
-    uint32_t* __restrict__ counts, const uint32_t n_tiles, uint32_t* __restrict__ totals
+    uint32_t* __restrict__ counts, const uint32_t bins, const uint32_t n_tiles, uint32_t* __restrict__ totals
 ) {
     const uint32_t lane = threadIdx.x;
-    uint32_t* row = counts + (size_t) blockIdx.x * n_tiles;
     uint32_t carry = 0;
     for (uint32_t t0 = 0; t0 < n_tiles; t0 += 64 * 4) {
         uint32_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t t = t0 + j * 64 + lane;
-            v[j] = t < n_tiles ? row[t] : 0;
+            v[j] = t < n_tiles ? counts[(size_t) t * bins + blockIdx.x] : 0;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t t = t0 + j * 64 + lane;
             const uint32_t incl = wave_inclusive_sum(v[j], lane);
-            if (t < n_tiles) row[t] = carry + incl - v[j];
+            if (t < n_tiles) counts[(size_t) t * bins + blockIdx.x] = carry + incl - v[j];
             carry += __shfl(incl, 63);
         }
     }
     if (lane == 0) totals[blockIdx.x] = carry;
 }
 
-// Exclusive sums of `bins` totals into base[] (LDS), by a workgroup of 256.
-__device__ __forceinline__ void scan_totals(const uint32_t* totals, const uint32_t bins, uint32_t* base, uint32_t* wave_sum) {
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t each = (bins + 255) / 256, from = min(tid * each, bins), to = min(from + each, bins);
-    uint32_t mine = 0;
-    for (uint32_t b = from; b < to; ++b) mine += totals[b];
-    const uint32_t incl = wave_inclusive_sum(mine, lane);
-    if (lane == 63) wave_sum[wave] = incl;
-    __syncthreads();
-    uint32_t running = incl - mine;
-    for (uint32_t w = 0; w < wave; ++w) running += wave_sum[w];
-    for (uint32_t b = from; b < to; ++b) {
-        base[b] = running;
-        running += totals[b];
-    }
-    __syncthreads();
-}
-
-constexpr int PLACE_PER_THREAD = 4;
-
-// Third launch: every element's place.  A radix pass moves its key and its index there; the only pass of a route writes
-// the slots, the order and the offsets instead (bin `bins - 1` then holds the dropped choices).
-template <bool ROUTE>
-__global__ __launch_bounds__(256) void place_kernel(
-    const KeySource source, const size_t n, const int shift, const uint32_t mask, const uint32_t bins, const uint32_t tile,
+// Last launch: the elements of a tile to their places.  SCANNED: the counts are those of the tiles before already.
+template <bool ROUTE, bool SCANNED>
+__global__ __launch_bounds__(SORT_THREADS) void place_kernel(
+    const KeySource source, const size_t n, const int shift, const uint32_t mask, const uint32_t bins, const uint32_t rounds,
     const uint32_t n_tiles, const uint16_t* __restrict__ ranks, const uint32_t* __restrict__ counts,
-    const uint32_t* __restrict__ totals, const uint32_t* __restrict__ index_in, uint32_t* __restrict__ keys_out,
-    uint32_t* __restrict__ index_out, uint32_t* __restrict__ slots, uint32_t* __restrict__ order, uint32_t* __restrict__ offsets
+    const uint32_t* __restrict__ totals, const Places places
 ) {
     __shared__ uint32_t base[MAX_BINS];
-    __shared__ uint32_t wave_sum[4];
-    scan_totals(totals, bins, base, wave_sum);
-    if (ROUTE && blockIdx.x == 0)
-        for (uint32_t b = threadIdx.x; b < bins; b += 256) offsets[b] = base[b];
-#pragma unroll
-    for (int j = 0; j < PLACE_PER_THREAD; ++j) {
-        const size_t i = ((size_t) blockIdx.x * PLACE_PER_THREAD + j) * 256 + threadIdx.x;
-        if (i >= n) continue;
-        const uint32_t key = source(i), digit = (key >> shift) & mask;
-        const uint32_t place = base[digit] + counts[(size_t) digit * n_tiles + (uint32_t) (i / tile)] + ranks[i];
-        if (ROUTE) {
-            const bool kept = key < source.limit;
-            slots[i] = kept ? place : SKM_NO_ROW;
-            if (order) order[place] = kept ? (uint32_t) i : SKM_NO_ROW;
+    __shared__ uint32_t wave_sum[SORT_WAVES];
+    const uint32_t tid = threadIdx.x, tile = blockIdx.x;
+    uint32_t before = 0, total = 0;
+    if (tid < bins) {
+        if (SCANNED) {
+            before = counts[(size_t) tile * bins + tid];
+            total = totals[tid];
         } else {
-            keys_out[place] = key;
-            index_out[place] = index_in ? index_in[i] : (uint32_t) i;
+#pragma unroll 8
+            for (uint32_t t = 0; t < n_tiles; ++t) {
+                const uint32_t c = counts[(size_t) t * bins + tid];
+                total += c;
+                before += t < tile ? c : 0;
+            }
         }
+    }
+    const uint32_t start = block_exclusive_sum(total, wave_sum);
+    if (tid < bins) {
+        base[tid] = start + before;
+        if (ROUTE && tile == 0) places.offsets[tid] = start;
+    }
+    __syncthreads();
+    for (uint32_t r = 0; r < rounds; ++r) {
+        const size_t i = ((size_t) tile * rounds + r) * SORT_THREADS + tid;
+        if (i >= n) return;
+        const uint32_t key = source(i);
+        places.put<ROUTE>(i, key, source.limit, base[(key >> shift) & mask] + ranks[i]);
     }
 }
 
@@ -182,71 +234,6 @@ __global__ __launch_bounds__(256) void route_places_kernel(
     if (order) order[p] = kept ? index[p] : SKM_NO_ROW;
 }
 
-// A whole route in one workgroup of 16 wavefronts, each with a contiguous share of the choices and counters of its own:
-// a decoding step's few thousand choices cost one launch instead of three.
-constexpr uint32_t ONE_LAUNCH_BINS = 1024, ONE_LAUNCH_ROUNDS = 8;
-constexpr size_t ONE_LAUNCH_CHOICES = (size_t) 1024 * ONE_LAUNCH_ROUNDS;
-
-template <int ROUNDS>
-__global__ __launch_bounds__(1024) void route_one_launch_kernel(
-    const uint32_t* __restrict__ choices, const uint32_t n, const uint32_t groups, const int bits, uint32_t* __restrict__ slots,
-    uint32_t* __restrict__ order, uint32_t* __restrict__ offsets
-) {
-    extern __shared__ uint16_t count16[];  // [16][groups + 1]; no count passes ONE_LAUNCH_CHOICES
-    __shared__ uint32_t wave_sum[16];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = groups + 1;
-    for (uint32_t b = tid; b < 16 * bins; b += 1024) count16[b] = 0;
-    __syncthreads();
-    uint16_t* mine = count16 + wave * bins;
-    const uint32_t first = wave * ROUNDS * 64;
-    uint32_t key[ROUNDS], rank[ROUNDS];
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const uint32_t i = first + r * 64 + lane;
-        key[r] = i < n ? choices[i] : 0;
-        key[r] = key[r] < groups ? key[r] : groups;
-    }
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const bool in = first + r * 64 + lane < n;
-        const unsigned long long match = equal_lanes(in, key[r], bits);
-        const uint32_t below = (uint32_t) __popcll(match & lanes_below(lane));
-        const uint32_t before = in ? mine[key[r]] : 0;
-        rank[r] = before + below;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wavefront's LDS accesses stay in this order
-        if (in && below == 0) mine[key[r]] = (uint16_t) (before + __popcll(match));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    __syncthreads();
-    // thread b: the counts of bin b in the wavefronts before, then the bins before
-    uint32_t total = 0;
-    if (tid < bins)
-        for (int w = 0; w < 16; ++w) {
-            const uint32_t c = count16[w * bins + tid];
-            count16[w * bins + tid] = (uint16_t) total;
-            total += c;
-        }
-    const uint32_t incl = wave_inclusive_sum(total, lane);
-    if (lane == 63) wave_sum[wave] = incl;
-    __syncthreads();
-    uint32_t base = incl - total;
-    for (uint32_t w = 0; w < wave; ++w) base += wave_sum[w];
-    if (tid < bins) {
-        offsets[tid] = base;
-        for (int w = 0; w < 16; ++w) count16[w * bins + tid] += (uint16_t) base;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const uint32_t i = first + r * 64 + lane;
-        if (i >= n) continue;
-        const uint32_t place = mine[key[r]] + rank[r];
-        const bool kept = key[r] < groups;
-        slots[i] = kept ? place : SKM_NO_ROW;
-        if (order) order[place] = kept ? i : SKM_NO_ROW;
-    }
-}
-
 int bits_for(const uint64_t bins) {
     int bits = 1;
     while ((uint64_t(1) << bits) < bins) ++bits;
@@ -260,18 +247,21 @@ struct SortPlan {
     size_t n;
     uint32_t limit;
     int passes, bits_per_pass;
-    uint32_t bins, rounds, tile, n_tiles;
+    uint32_t bins, rounds, n_tiles;
     size_t at_ranks, at_counts, at_totals, at_keys[2], at_index[2], bytes;
 
-    SortPlan(const size_t n_, const size_t limit_, const bool one_pass_moves_nothing) : n(n_), limit((uint32_t) limit_) {
+    SortPlan(const size_t n_, const size_t limit_, const bool route) : n(n_), limit((uint32_t) limit_) {
         const int bits = bits_for((uint64_t) limit + 1);
         passes = (bits + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS;
         bits_per_pass = (bits + passes - 1) / passes;
         bins = passes == 1 ? limit + 1 : 1u << bits_per_pass;
-        // a short tile spreads few keys over many wavefronts; with many keys a tile has at least as many elements as
-        // there are digit values, so that the counts take no more memory than the keys
-        rounds = n <= (size_t(1) << 20) ? 8 : std::max<uint32_t>(8, bins / 64);
-        tile = rounds * 64;
+        // short tiles spread few keys over many compute units; more than 32 tiles bring nothing
+        rounds = 1;
+        while (rounds < MAX_ROUNDS && (size_t) SORT_THREADS * rounds * 32 < n) rounds *= 2;
+        const bool only = route && passes == 1 && n <= (size_t) SORT_THREADS * MAX_ROUNDS;
+        if (only)
+            while ((size_t) SORT_THREADS * rounds < n) rounds *= 2;
+        const uint32_t tile = SORT_THREADS * rounds;
         n_tiles = (uint32_t) ((n + tile - 1) / tile);
         size_t at = 0;
         const auto take = [&](const size_t bytes) {
@@ -279,10 +269,13 @@ struct SortPlan {
             at += aligned(bytes);
             return here;
         };
-        at_ranks = take(n * 2);
-        at_counts = take((size_t) bins * n_tiles * 4);
-        at_totals = take((size_t) bins * 4);
-        const bool moves = passes > 1 || !one_pass_moves_nothing;
+        at_ranks = at_counts = at_totals = 0;
+        if (!only) {
+            at_ranks = take(n * 2);
+            at_counts = take((size_t) bins * n_tiles * 4);
+            at_totals = take((size_t) bins * 4);
+        }
+        const bool moves = passes > 1 || !route;
         for (int b = 0; b < 2; ++b) {
             at_keys[b] = moves && (b == 0 || passes > 1) ? take(n * 4) : 0;
             at_index[b] = moves && (b == 0 || passes > 1) ? take(n * 4) : 0;
@@ -292,38 +285,47 @@ struct SortPlan {
     int last() const { return (passes - 1) & 1; }  // which pair of arrays holds the result
 };
 
-struct RouteOut {
-    uint32_t *slots, *order, *offsets;
-};
-
 // Queues the passes of a sort; `route`: the single pass writes these instead of sorted keys.
-int launch_sort(skm_ctx* ctx, const SortPlan& p, const KeySource& first, char* scratch, const RouteOut* route) {
+int launch_sort(skm_ctx* ctx, const SortPlan& p, const KeySource& first, char* scratch, const Places* route) {
     uint16_t* ranks = (uint16_t*) (scratch + p.at_ranks);
     uint32_t* counts = (uint32_t*) (scratch + p.at_counts);
     uint32_t* totals = (uint32_t*) (scratch + p.at_totals);
-    const unsigned place_blocks = (unsigned) ((p.n + 256 * PLACE_PER_THREAD - 1) / (256 * PLACE_PER_THREAD));
     KeySource source = first;
-    const uint32_t* index_in = nullptr;
+    Places to{};
+    const size_t lds = (size_t) SORT_WAVES * p.bins * sizeof(uint16_t);
+    const int bits = bits_for(p.bins);
+    const bool scanned = p.n_tiles > TILES_WITHOUT_SCAN;
     for (int pass = 0; pass < p.passes; ++pass) {
         const int shift = pass * p.bits_per_pass;
         const uint32_t mask = p.passes == 1 ? 0xffffffffu : p.bins - 1;
-        tile_ranks_kernel<<<p.n_tiles, 64, p.bins * 4, ctx->stream>>>(source, p.n, shift, mask, bits_for(p.bins), p.bins, p.rounds,
-                                                                     p.n_tiles, ranks, counts);
-        SKM_TRY(check_hip(hipGetLastError(), "tile_ranks_kernel launch"));
-        tile_counts_scan_kernel<<<p.bins, 64, 0, ctx->stream>>>(counts, p.n_tiles, totals);
-        SKM_TRY(check_hip(hipGetLastError(), "tile_counts_scan_kernel launch"));
-        uint32_t* keys_out = (uint32_t*) (scratch + p.at_keys[pass & 1]);
-        uint32_t* index_out = (uint32_t*) (scratch + p.at_index[pass & 1]);
-        if (route)
-            place_kernel<true><<<place_blocks, 256, 0, ctx->stream>>>(source, p.n, shift, mask, p.bins, p.tile, p.n_tiles, ranks, counts,
-                                                                      totals, nullptr, nullptr, nullptr, route->slots, route->order,
-                                                                      route->offsets);
-        else
-            place_kernel<false><<<place_blocks, 256, 0, ctx->stream>>>(source, p.n, shift, mask, p.bins, p.tile, p.n_tiles, ranks, counts,
-                                                                       totals, index_in, keys_out, index_out, nullptr, nullptr, nullptr);
-        SKM_TRY(check_hip(hipGetLastError(), "place_kernel launch"));
-        source = KeySource{keys_out, SKM_U32, p.limit};
-        index_in = index_out;
+        if (route) {
+            to = *route;
+        } else {
+            to.index_in = to.index;
+            to.keys = (uint32_t*) (scratch + p.at_keys[pass & 1]);
+            to.index = (uint32_t*) (scratch + p.at_index[pass & 1]);
+        }
+        const bool only = route && p.n_tiles == 1 && p.at_totals == 0;
+        const auto rank = [&](auto rounds) {
+            constexpr int R = decltype(rounds)::value;
+            if (only) tile_ranks_kernel<R, true><<<1, SORT_THREADS, lds, ctx->stream>>>(source, p.n, shift, mask, bits, p.bins, ranks, counts, to);
+            else tile_ranks_kernel<R, false><<<p.n_tiles, SORT_THREADS, lds, ctx->stream>>>(source, p.n, shift, mask, bits, p.bins, ranks, counts, to);
+            return check_hip(hipGetLastError(), "tile_ranks_kernel launch");
+        };
+        SKM_TRY(p.rounds == 1 ? rank(std::integral_constant<int, 1>{}) : p.rounds == 2 ? rank(std::integral_constant<int, 2>{})
+                : p.rounds == 4 ? rank(std::integral_constant<int, 4>{}) : rank(std::integral_constant<int, 8>{}));
+        if (only) return SKM_OK;
+        if (scanned) {
+            tile_counts_scan_kernel<<<p.bins, 64, 0, ctx->stream>>>(counts, p.bins, p.n_tiles, totals);
+            SKM_TRY(check_hip(hipGetLastError(), "tile_counts_scan_kernel launch"));
+        }
+        const auto place = [&](auto kernel) {
+            kernel<<<p.n_tiles, SORT_THREADS, 0, ctx->stream>>>(source, p.n, shift, mask, p.bins, p.rounds, p.n_tiles, ranks, counts, totals, to);
+            return check_hip(hipGetLastError(), "place_kernel launch");
+        };
+        if (route) SKM_TRY(scanned ? place(place_kernel<true, true>) : place(place_kernel<true, false>));
+        else SKM_TRY(scanned ? place(place_kernel<false, true>) : place(place_kernel<false, false>));
+        source = KeySource{to.keys, SKM_U32, p.limit};
     }
     return SKM_OK;
 }
@@ -332,25 +334,6 @@ int launch_sort(skm_ctx* ctx, const SortPlan& p, const KeySource& first, char* s
 // Gradient of a lookup
 // ---------------------------------------------------------------------------------------------
 
-constexpr int GRAD_AHEAD = 4;  // token rows requested before the first is added
-
-// Adds the grad rows of the tokens at [j0, j1) of `index` (sorted order) to sum; `at`: the lane's vector in the row.
-template <class T, int E>
-__device__ __forceinline__ void add_tokens(const T* __restrict__ grad, const size_t stride, const uint32_t* __restrict__ index,
-                                           const uint32_t j0, const uint32_t j1, const uint32_t at, vec_of<float, E>& sum) {
-    for (uint32_t j = j0; j < j1; j += GRAD_AHEAD) {
-        vec_of<T, E> v[GRAD_AHEAD];
-#pragma unroll
-        for (int q = 0; q < GRAD_AHEAD; ++q) {
-            const uint32_t i = index[min(j + q, j1 - 1)];
-            v[q] = load_vec<T, E>(grad + (size_t) i * stride + (size_t) at * E);
-        }
-#pragma unroll
-        for (int q = 0; q < GRAD_AHEAD; ++q)
-            if (j + q < j1) sum += widen<E>(v[q]);
-    }
-}
-
 template <class O, int E>
 __device__ __forceinline__ void put_sum(O* to, const vec_of<float, E> sum, const float scale, const bool accumulate) {
     vec_of<float, E> r = sum * scale;
@@ -358,132 +341,309 @@ __device__ __forceinline__ void put_sum(O* to, const vec_of<float, E> sum, const
     store_vec<O, E>(to, narrow<O, E>(r));
 }
 
-// Table rows of at most `most` tokens: a sum each, or zeros where there are none (nothing when accumulating).
-template <class T, class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_rows_kernel(
-    const T* __restrict__ grad, const size_t grad_stride, const uint32_t* __restrict__ index, const uint32_t* __restrict__ offsets,
-    const size_t rows, const uint32_t most, const float scale, O* __restrict__ out, const size_t out_stride, const int accumulate,
-    const RowSplit s
-) {
-    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
-    const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
-    for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
-        const size_t row = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
-        const uint32_t at = (uint32_t) (u % s.pieces) * s.lanes + in_row;
-        if (row >= rows || at >= s.vectors) continue;
-        const uint32_t j0 = offsets[row], j1 = offsets[row + 1];
-        if (j1 - j0 > most || (accumulate && j0 == j1)) continue;
-        vec_of<float, E> sum = {};
-        add_tokens<T, E>(grad, grad_stride, index, j0, j1, at, sum);
-        put_sum<O, E>(out + row * out_stride + (size_t) at * E, sum, scale, accumulate);
-    }
-}
+struct GradArgs {
+    const void* grad;
+    size_t grad_stride;
+    void* out;
+    size_t out_stride;
+    float scale;
+    int accumulate;
+    uint32_t n, rows, vectors, pieces;  // vectors per row; pieces of 64 vectors
+    // sorted tokens: their keys and positions, in chunks of `chunk`, and the chunks' sums of rows that go past them
+    const uint32_t *keys, *index;
+    uint32_t chunk, chunks;
+    float* parts;
+};
 
-// Rows of more tokens than that: the sorted tokens are cut into chunks of `most`.  A chunk leaves at most two sums: of the
-// row that its first token belongs to (slot 0) and of another one that its last token belongs to (slot 1), as far
-// as they are such long rows.
-template <class T, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_chunks_kernel(
-    const T* __restrict__ grad, const size_t grad_stride, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ index,
-    const uint32_t* __restrict__ offsets, const uint32_t n, const uint32_t rows, const uint32_t most, float* __restrict__ parts,
-    const uint32_t vectors, const uint32_t pieces, const uint32_t chunks
-) {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6);
-    if (u >= (uint64_t) chunks * pieces) return;
-    const uint32_t c = (uint32_t) (u / pieces), at = (uint32_t) (u % pieces) * 64 + lane;
-    if (at >= vectors) return;
-    const uint32_t from = c * most, to = (uint32_t) min((uint64_t) n, (uint64_t) from + most);
-    const uint32_t head = keys[from], tail = keys[to - 1];
-    float* part = parts + (size_t) c * 2 * vectors * E + (size_t) at * E;
-    if (head < rows && offsets[head + 1] - offsets[head] > most) {
-        vec_of<float, E> sum = {};
-        add_tokens<T, E>(grad, grad_stride, index, from, min(to, offsets[head + 1]), at, sum);
-        store_vec<float, E>(part, sum);
-    }
-    if (tail < rows && offsets[tail] > from && offsets[tail + 1] - offsets[tail] > most) {
-        vec_of<float, E> sum = {};
-        add_tokens<T, E>(grad, grad_stride, index, offsets[tail], to, at, sum);
-        store_vec<float, E>(part + (size_t) vectors * E, sum);
-    }
-}
-
-// The long row that begins in a chunk (a row of more than `most` tokens covers the end of the chunk it begins in, so
-// there is at most one): its chunks' sums added up in order.
-template <class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ offsets, const uint32_t n, const uint32_t rows, const uint32_t most,
-    const float* __restrict__ parts, const float scale, O* __restrict__ out, const size_t out_stride, const int accumulate,
-    const uint32_t vectors, const uint32_t pieces, const uint32_t chunks
-) {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6);
-    if (u >= (uint64_t) chunks * pieces) return;
-    const uint32_t c = (uint32_t) (u / pieces), at = (uint32_t) (u % pieces) * 64 + lane;
-    if (at >= vectors) return;
-    const uint32_t from = c * most, to = (uint32_t) min((uint64_t) n, (uint64_t) from + most);
-    const uint32_t row = keys[to - 1];
-    if (row >= rows || offsets[row] < from || offsets[row + 1] - offsets[row] <= most) return;
-    const uint32_t last = (offsets[row + 1] - 1) / most;
-    const size_t chunk = (size_t) 2 * vectors * E;
-    const float* part = parts + (size_t) at * E;
-    vec_of<float, E> sum = load_vec<float, E>(part + c * chunk + (offsets[row] == from ? 0 : (size_t) vectors * E));
-    for (uint32_t i = c + 1; i <= last; ++i) sum += load_vec<float, E>(part + i * chunk);
-    put_sum<O, E>(out + (size_t) row * out_stride + (size_t) at * E, sum, scale, accumulate);
-}
-
-// Few tokens: no sort.  The first token of every id looks through the others for the same id and adds them in order; the
-// table was set to zeros before (unless accumulating).
-constexpr size_t FEW_TOKENS = 2048;
+// The sorted tokens are cut into chunks, so that however the ids are spread every wavefront adds up the same number of tokens,
+// GRAD_AHEAD of them on their way before the first is added.  A row whose tokens are all in a chunk is stored; of the
+// rows that began before the chunk or go on after it, at most two, the sum of this chunk's tokens goes to `parts`: slot 0 if
+// the row holds the chunk's first token, else slot 1.  Rows of few vectors share a wavefront: `lanes` lanes to a chunk.
+constexpr int GRAD_AHEAD = 8, GRAD_VECTORS = 2;  // vectors a lane holds of a row
 
 template <class T, class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_few_kernel(
-    const T* __restrict__ grad, const size_t grad_stride, const KeySource source, const uint32_t n, const float scale,
-    O* __restrict__ out, const size_t out_stride, const int accumulate, const uint32_t vectors, const uint32_t pieces
-) {
+__device__ __forceinline__ void grad_of_chunk(const GradArgs& g, const RowSplit& s, const uint64_t unit) {
+    const T* grad = reinterpret_cast<const T*>(g.grad);
     const uint32_t lane = threadIdx.x & 63;
-    const uint32_t u = blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6);
-    if (u >= n * pieces) return;
-    const uint32_t t = u / pieces, at = (u % pieces) * 64 + lane;
-    const uint32_t id = source(t);
-    if (id == source.limit) return;
-    bool earlier = false;
-    for (uint32_t s = lane; s < t; s += 64) earlier |= source(s) == id;
-    if (__ballot(earlier)) return;
-    vec_of<float, E> sum = {};
-    for (uint32_t s0 = t / 64 * 64; s0 < n; s0 += 64) {
-        const uint32_t s = s0 + lane;
-        unsigned long long same = __ballot(s >= t && s < n && source(s) == id);
-        while (same) {
-            const uint32_t i = s0 + (uint32_t) __builtin_ctzll(same);
-            same &= same - 1;
-            if (at < vectors) sum += widen<E>(load_vec<T, E>(grad + (size_t) i * grad_stride + (size_t) at * E));
+    const uint64_t c = unit / s.pieces * (64 / s.lanes) + lane / s.lanes;
+    if (c >= g.chunks) return;
+    const uint32_t first = (uint32_t) (unit % s.pieces) * s.lanes * GRAD_VECTORS + (lane & (s.lanes - 1));
+    const uint32_t from = (uint32_t) c * g.chunk, to = (uint32_t) min((uint64_t) g.n, (uint64_t) from + g.chunk);
+    uint32_t row = g.keys[from];
+    if (row >= g.rows) return;  // nobody's tokens are at the end
+    const bool goes_on = to < g.n && g.keys[to] == g.keys[to - 1];
+    bool whole = from == 0 || g.keys[from - 1] != row;  // the row began in this chunk
+    int slot = 0;
+    vec_of<float, E> sum[GRAD_VECTORS] = {};
+    const auto put = [&](const bool ends) {
+#pragma unroll
+        for (int i = 0; i < GRAD_VECTORS; ++i) {
+            const uint32_t at = first + i * s.lanes;
+            if (at < g.vectors) {
+                if (whole && ends) put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) row * g.out_stride + (size_t) at * E, sum[i], g.scale, g.accumulate);
+                else store_vec<float, E>(g.parts + ((size_t) c * 2 + slot) * g.vectors * E + (size_t) at * E, sum[i]);
+            }
+            sum[i] = vec_of<float, E>{};
+        }
+        whole = true;
+        slot = 1;
+    };
+    for (uint32_t j = from; j < to; j += GRAD_AHEAD) {
+        vec_of<T, E> v[GRAD_AHEAD][GRAD_VECTORS];
+        uint32_t key[GRAD_AHEAD], token[GRAD_AHEAD];
+#pragma unroll
+        for (int q = 0; q < GRAD_AHEAD; ++q) {
+            key[q] = g.keys[min(j + q, to - 1)];
+            token[q] = g.index[min(j + q, to - 1)];
+        }
+#pragma unroll
+        for (int q = 0; q < GRAD_AHEAD; ++q)
+#pragma unroll
+            for (int i = 0; i < GRAD_VECTORS; ++i) {
+                const uint32_t at = first + i * s.lanes;
+                if (at < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) token[q] * g.grad_stride + (size_t) at * E);
+            }
+#pragma unroll
+        for (int q = 0; q < GRAD_AHEAD; ++q) {
+            if (j + q >= to) break;
+            if (key[q] != row) {
+                put(true);
+                row = key[q];
+                if (row >= g.rows) return;
+            }
+#pragma unroll
+            for (int i = 0; i < GRAD_VECTORS; ++i)
+                if (first + i * s.lanes < g.vectors) sum[i] += widen<E>(v[q][i]);
         }
     }
-    if (at < vectors) put_sum<O, E>(out + (size_t) id * out_stride + (size_t) at * E, sum, scale, accumulate);
+    put(!goes_on);
 }
 
+// Zeros for the rows without a token: a lane each finds whether its row has one (a binary search in the sorted keys), then the
+// wavefront stores the rows that have none one after the other.
+constexpr uint32_t FILL_ROWS = 16;
+
 template <class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void zero_rows_kernel(O* __restrict__ out, const size_t rows, const size_t stride, const RowSplit s) {
-    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
-    const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
-    for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
-        const size_t row = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
-        const uint32_t at = (uint32_t) (u % s.pieces) * s.lanes + in_row;
-        if (row < rows && at < s.vectors) store_vec<O, E>(out + row * stride + (size_t) at * E, vec_of<O, E>{});
+__device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit) {
+    const uint32_t lane = threadIdx.x & 63, row = unit * FILL_ROWS + lane;
+    bool empty = false;
+    if (lane < FILL_ROWS && row < g.rows) {
+        uint32_t low = 0, high = g.n;
+        while (low < high) {
+            const uint32_t mid = low + (high - low) / 2;
+            if (g.keys[mid] < row) low = mid + 1;
+            else high = mid;
+        }
+        empty = low == g.n || g.keys[low] != row;
+    }
+    for (unsigned long long left = __ballot(empty); left; left &= left - 1) {
+        O* out = reinterpret_cast<O*>(g.out) + (size_t) (unit * FILL_ROWS + (uint32_t) __builtin_ctzll(left)) * g.out_stride;
+        for (uint32_t at = lane; at < g.vectors; at += 64) store_vec<O, E>(out + (size_t) at * E, vec_of<O, E>{});
     }
 }
 
-// Scratch of the sorted path: the sort, the rows' offsets, the chunks' sums.
+// One launch for both: the chunks, whose wavefronts wait for memory, under the fill.
+template <class T, class O, int E>
+__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_kernel(const GradArgs g, const RowSplit s, const uint32_t chunk_blocks) {
+    const uint32_t wave = threadIdx.x >> 6;
+    if (blockIdx.x < chunk_blocks) {
+        const uint64_t unit = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + wave;
+        if (unit < s.units) grad_of_chunk<T, O, E>(g, s, unit);
+    } else {
+        const uint64_t unit = (uint64_t) (blockIdx.x - chunk_blocks) * (ROWS_THREADS / 64) + wave;
+        if (unit * FILL_ROWS < g.rows) fill_rows<O, E>(g, (uint32_t) unit);
+    }
+}
+
+// The row that begins in chunk c and goes on after it, and how many chunks have a sum of it (0: there is none).  All lanes
+// of a wavefront ask for the same chunk.
+struct Crossing {
+    uint32_t row, parts;
+    bool at_start;  // it begins with the chunk: the sum is in slot 0, else in slot 1
+};
+__device__ __forceinline__ Crossing crossing_row(const GradArgs& g, const uint32_t c) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t from = (uint64_t) c * g.chunk, to = from + g.chunk;
+    Crossing x{0, 0, false};
+    if (to >= g.n) return x;
+    const uint32_t before = g.keys[from > 0 ? from - 1 : 0], head = g.keys[from], tail = g.keys[to - 1], next = g.keys[to];
+    x.row = tail;
+    x.at_start = head == tail;
+    if (tail >= g.rows || next != tail || (x.at_start && from > 0 && before == tail)) return x;
+    x.parts = 1;
+    for (uint32_t d0 = c + 1;; d0 += 64) {  // the following chunks whose first token is the row's
+        const uint64_t first = (uint64_t) (d0 + lane) * g.chunk;
+        const unsigned long long other = ~__ballot(first < g.n && g.keys[first < g.n ? first : 0] == x.row);
+        x.parts += other ? (uint32_t) __builtin_ctzll(other) : 64;
+        if (other) return x;
+    }
+}
+
+// Adds up the chunks' sums of the rows that go past a chunk.  A row of at most JOIN_ALONE sums takes one wavefront (the first
+// `alone_blocks` workgroups), a longer one a workgroup, whose wavefronts take contiguous shares, added in order: such rows
+// begin at least JOIN_ALONE chunks apart, so a workgroup looks for the one of JOIN_ALONE chunks.
+constexpr uint32_t JOIN_ALONE = 16;
+
+template <class O, int E>
+__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(const GradArgs g, const uint32_t alone_blocks) {
+    constexpr int WAVES = ROWS_THREADS / 64;
+    __shared__ vec_of<float, E> share[WAVES][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t stride = (size_t) 2 * g.vectors * E;
+    uint32_t c, piece;
+    Crossing x;
+    const bool alone = blockIdx.x < alone_blocks;
+    if (alone) {
+        const uint64_t unit = (uint64_t) blockIdx.x * WAVES + wave;
+        if (unit >= (uint64_t) g.chunks * g.pieces) return;
+        c = (uint32_t) (unit / g.pieces), piece = (uint32_t) (unit % g.pieces);
+        x = crossing_row(g, c);
+        if (x.parts == 0 || x.parts > JOIN_ALONE) return;
+    } else {
+        const uint32_t unit = blockIdx.x - alone_blocks, c0 = unit / g.pieces * JOIN_ALONE;
+        piece = unit % g.pieces;
+        // lane i < JOIN_ALONE: does a row begin in chunk c0 + i that holds the first token of the JOIN_ALONE chunks after it
+        const uint64_t from = (uint64_t) (c0 + lane) * g.chunk, far = from + (uint64_t) JOIN_ALONE * g.chunk;
+        bool here = lane < JOIN_ALONE && far < g.n;
+        if (here) {
+            const uint32_t row = g.keys[far];
+            here = row < g.rows && g.keys[from + g.chunk - 1] == row && !(from > 0 && g.keys[from - 1] == row && g.keys[from] == row);
+        }
+        const unsigned long long which = __ballot(here);
+        if (!which) return;
+        c = c0 + (uint32_t) __builtin_ctzll(which);
+        x = crossing_row(g, c);
+    }
+    const uint32_t at = piece * 64 + lane;
+    const uint32_t each = alone ? x.parts : (x.parts + WAVES - 1) / WAVES;
+    const uint32_t p0 = alone ? 0 : min(wave * each, x.parts), p1 = min(p0 + each, x.parts);
+    vec_of<float, E> sum = {};
+    if (at < g.vectors) {
+        const float* part = g.parts + c * stride + (size_t) at * E;
+#pragma unroll 8
+        for (uint32_t p = p0; p < p1; ++p) sum += load_vec<float, E>(part + p * stride + (p == 0 && !x.at_start ? stride / 2 : 0));
+    }
+    if (!alone) {
+        share[wave][lane] = sum;
+        __syncthreads();
+        for (int w = 1; w < WAVES && wave == 0; ++w) sum += share[w][lane];
+    }
+    if ((alone || wave == 0) && at < g.vectors)
+        put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + (size_t) at * E, sum, g.scale, g.accumulate);
+}
+
+// Few tokens: one launch and no sort.  A workgroup owns every `step`-th row, reads all ids, and lists the tokens of its rows in order
+// (every wavefront those of a contiguous share).  Then its wavefronts take the rows one by one, and together those of
+// many tokens, each wavefront the tokens of its share.
+constexpr size_t FEW_TOKENS = 2048;
+constexpr int FEW_THREADS = 512, FEW_AHEAD = 4;
+constexpr uint32_t FEW_ROWS = 64;  // of a workgroup, at most
+constexpr uint32_t FEW_MOST = 8;   // tokens of a row that one wavefront adds up
+
+template <class T, class O, int E>
+__global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const GradArgs g, const KeySource source, const uint32_t step) {
+    constexpr int WAVES = FEW_THREADS / 64, SHARE = FEW_TOKENS / WAVES, V = E >= 8 ? 2 : 4;  // V: vectors a lane holds of a row
+    __shared__ uint32_t listed[WAVES][SHARE];  // number of the row, token
+    __shared__ uint32_t many[WAVES], of_row[FEW_ROWS];
+    __shared__ vec_of<float, E> share[WAVES][V][64];
+    const T* grad = reinterpret_cast<const T*>(g.grad);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t mine = (g.rows - blockIdx.x + step - 1) / step;  // rows blockIdx.x, + step, ...
+    if (threadIdx.x < FEW_ROWS) of_row[threadIdx.x] = 0;
+    uint32_t id[SHARE / 64];
+#pragma unroll
+    for (int q = 0; q < SHARE / 64; ++q) {
+        const uint32_t t = wave * SHARE + q * 64 + lane;
+        id[q] = t < g.n ? source(t) : source.limit;
+    }
+    __syncthreads();
+    uint32_t count = 0;
+#pragma unroll
+    for (int q = 0; q < SHARE / 64; ++q) {
+        const uint32_t r = id[q] / step;
+        const bool here = id[q] < source.limit && id[q] - r * step == blockIdx.x;
+        const unsigned long long who = __ballot(here);
+        if (here) {
+            listed[wave][count + (uint32_t) __popcll(who & lanes_below(lane))] = r << 16 | (wave * SHARE + q * 64 + lane);
+            atomicAdd(&of_row[r], 1u);
+        }
+        count += (uint32_t) __popcll(who);
+    }
+    if (lane == 0) many[wave] = count;
+    __syncthreads();
+    // adds the tokens of row r in the w-th share; `at`: the lane's first vector, the others 64 apart
+    const auto add_share = [&](const uint32_t w, const uint32_t r, const uint32_t at, vec_of<float, E> (&sum)[V]) {
+        for (uint32_t k0 = 0; k0 < many[w]; k0 += 64) {
+            const uint32_t entry = k0 + lane < many[w] ? listed[w][k0 + lane] : 0xffffffffu;
+            unsigned long long same = __ballot(entry >> 16 == r);
+            while (same) {
+                vec_of<T, E> v[FEW_AHEAD][V];
+                int taken = 0;
+#pragma unroll
+                for (int q = 0; q < FEW_AHEAD; ++q) {
+                    if (same) {
+                        const uint32_t t = __builtin_amdgcn_readlane(entry, __builtin_ctzll(same)) & 0xffffu;
+                        same &= same - 1;
+#pragma unroll
+                        for (int i = 0; i < V; ++i)
+                            if (at + i * 64 < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) t * g.grad_stride + (size_t) (at + i * 64) * E);
+                        taken = q + 1;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < FEW_AHEAD; ++q)
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        if (q < taken && at + i * 64 < g.vectors) sum[i] += widen<E>(v[q][i]);
+            }
+        }
+    };
+    const auto put = [&](const uint32_t r, const uint32_t at, const vec_of<float, E> (&sum)[V]) {
+        O* out = reinterpret_cast<O*>(g.out) + (size_t) (r * step + blockIdx.x) * g.out_stride;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (at + i * 64 < g.vectors) put_sum<O, E>(out + (size_t) (at + i * 64) * E, sum[i], g.scale, g.accumulate);
+    };
+    const uint32_t pieces = (g.vectors + 64 * V - 1) / (64 * V);
+    for (uint32_t u = wave; u < mine * pieces; u += WAVES) {
+        const uint32_t r = u / pieces, at = u % pieces * (64 * V) + lane, tokens = of_row[r];
+        if (tokens > FEW_MOST || (g.accumulate && tokens == 0)) continue;
+        vec_of<float, E> sum[V] = {};
+        if (tokens)
+            for (uint32_t w = 0; w < WAVES; ++w) add_share(w, r, at, sum);
+        put(r, at, sum);
+    }
+    for (uint32_t r = 0; r < mine; ++r) {
+        if (of_row[r] <= FEW_MOST) continue;
+        for (uint32_t piece = 0; piece < pieces; ++piece) {
+            const uint32_t at = piece * (64 * V) + lane;
+            vec_of<float, E> sum[V] = {};
+            add_share(wave, r, at, sum);
+#pragma unroll
+            for (int i = 0; i < V; ++i) share[wave][i][lane] = sum[i];
+            __syncthreads();
+            if (wave == 0) {
+                for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] += share[w][i][lane];
+                put(r, at, sum);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Scratch of the sorted path: the sort and the chunks' sums.
 struct GradPlan {
     SortPlan sort;
-    uint32_t most, chunks;
-    size_t at_offsets, at_parts, bytes;
+    uint32_t chunk, chunks;
+    size_t at_parts, bytes;
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
-        most = n <= 32768 ? 64 : 256;
-        chunks = (uint32_t) ((n + most - 1) / most);
-        at_offsets = sort.bytes;
-        at_parts = at_offsets + aligned((rows + 1) * 4);
+        // The additions of a chunk, and of a row's chunks, are chains: longer chunks for more tokens keep the second short
+        // where many tokens are on one row.
+        chunk = n <= (size_t(1) << 17) ? 32 : n <= (size_t(1) << 20) ? 128 : 256;
+        chunks = (uint32_t) ((n + chunk - 1) / chunk);
+        at_parts = sort.bytes;
         bytes = at_parts + aligned((size_t) chunks * 2 * d * 4);
     }
 };
@@ -501,7 +661,7 @@ int skm_route_scratch(size_t n, size_t choices, size_t groups, size_t* out_bytes
     SKM_REQUIRE(choices > 0 && choices <= SKM_ROUTE_MAX_CHOICES, "choices out of range");
     SKM_REQUIRE(n <= SKM_ROUTE_MAX_PLACES / choices, "n * choices out of range");
     const size_t places = n * choices;
-    *out_bytes = places == 0 || (places <= ONE_LAUNCH_CHOICES && groups < ONE_LAUNCH_BINS) ? 0 : SortPlan(places, groups, true).bytes;
+    *out_bytes = places == 0 ? 0 : SortPlan(places, groups, true).bytes;
     return SKM_OK;
 }
 
@@ -519,23 +679,11 @@ int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices,
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/route");
     if (places == 0) return skm_fill_u32(ctx, d_offsets, 0, groups + 1);
-    if (places <= ONE_LAUNCH_CHOICES && groups < ONE_LAUNCH_BINS) {
-        const size_t lds = 16 * (groups + 1) * sizeof(uint16_t);
-        const int bits = bits_for(groups + 1);
-        const auto launch = [&](auto rounds) {
-            route_one_launch_kernel<decltype(rounds)::value><<<1, 1024, lds, ctx->stream>>>(
-                d_choices, (uint32_t) places, (uint32_t) groups, bits, d_slots, d_order, d_offsets);
-            return check_hip(hipGetLastError(), "route_one_launch_kernel launch");
-        };
-        if (places <= 1024) return launch(std::integral_constant<int, 1>{});
-        if (places <= 1024 * 3) return launch(std::integral_constant<int, 3>{});
-        return launch(std::integral_constant<int, ONE_LAUNCH_ROUNDS>{});
-    }
     const SortPlan plan(places, groups, true);
     void* scratch = nullptr;
     SKM_TRY(call_scratch(ctx, __func__, d_scratch, scratch_bytes, plan.bytes, &scratch));
     const KeySource source{d_choices, SKM_U32, (uint32_t) groups};
-    const RouteOut out{d_slots, d_order, d_offsets};
+    const Places out{nullptr, nullptr, nullptr, d_slots, d_order, d_offsets};
     if (plan.passes == 1) return launch_sort(ctx, plan, source, (char*) scratch, &out);
     SKM_TRY(launch_sort(ctx, plan, source, (char*) scratch, nullptr));
     const uint32_t* keys = (const uint32_t*) ((char*) scratch + plan.at_keys[plan.last()]);
@@ -572,29 +720,31 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
     SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_out, span(rows, out_stride, d, out_size)), "out overlaps the gradient");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup_grad");
-    // elements per lane: what the gradient's alignment gives in one load and the table's in stores of at most 16 bytes
+    // elements per lane: what the alignment of both sides gives in one load and one store of at most 16 bytes
     const size_t in_width = common_width({address(d_grad), grad_stride * size, d * size});
     const size_t out_width = common_width({address(d_out), out_stride * out_size, d * out_size});
-    size_t per_lane = in_width / size;
-    if (out_width < 16) per_lane = std::min(per_lane, out_width / out_size);
+    const size_t per_lane = std::min(in_width / size, out_width / out_size);
     const KeySource source{d_ids, ids_type, (uint32_t) rows};
     const auto run = [&](auto sample, auto out_sample) {
         using T = decltype(sample);
         using O = decltype(out_sample);
         return for_width<T>(per_lane * size, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const uint32_t vectors = (uint32_t) (d / E), pieces = (vectors + 63) / 64;
-            const RowSplit s = split_rows(rows, vectors, 1);
-            O* out = (O*) d_out;
+            GradArgs g{};
+            g.grad = d_grad;
+            g.grad_stride = grad_stride;
+            g.out = d_out;
+            g.out_stride = out_stride;
+            g.scale = scale;
+            g.accumulate = accumulate != 0;
+            g.n = (uint32_t) n;
+            g.rows = (uint32_t) rows;
+            g.vectors = (uint32_t) (d / E);
+            g.pieces = (g.vectors + 63) / 64;
             if (n <= FEW_TOKENS) {
-                if (!accumulate) {
-                    zero_rows_kernel<O, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(out, rows, out_stride, s);
-                    SKM_TRY(check_hip(hipGetLastError(), "zero_rows_kernel launch"));
-                }
-                if (n == 0) return (int) SKM_OK;
-                const unsigned blocks = (unsigned) ((n * pieces + ROWS_THREADS / 64 - 1) / (ROWS_THREADS / 64));
-                lookup_grad_few_kernel<T, O, E><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
-                    (const T*) d_grad, grad_stride, source, (uint32_t) n, scale, out, out_stride, accumulate, vectors, pieces);
+                // a workgroup per row up to 1,024, then a few rows each: reading the ids costs a workgroup about as much as two rows
+                const uint32_t step = (uint32_t) std::max<size_t>(std::min<size_t>(rows, 1024), (rows + FEW_ROWS - 1) / FEW_ROWS);
+                lookup_grad_few_kernel<T, O, E><<<step, FEW_THREADS, 0, ctx->stream>>>(g, source, step);
                 return check_hip(hipGetLastError(), "lookup_grad_few_kernel launch");
             }
             const GradPlan plan(n, rows, d);
@@ -602,24 +752,23 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
             SKM_TRY(call_scratch(ctx, "skm_lookup_rows_grad", d_scratch, scratch_bytes, plan.bytes, &at));
             char* scratch = (char*) at;
             SKM_TRY(launch_sort(ctx, plan.sort, source, scratch, nullptr));
-            const uint32_t* keys = (const uint32_t*) (scratch + plan.sort.at_keys[plan.sort.last()]);
-            const uint32_t* index = (const uint32_t*) (scratch + plan.sort.at_index[plan.sort.last()]);
-            uint32_t* offsets = (uint32_t*) (scratch + plan.at_offsets);
-            float* parts = (float*) (scratch + plan.at_parts);
-            key_bounds_kernel<<<(unsigned) (rows / 256 + 1), 256, 0, ctx->stream>>>(keys, (uint32_t) n, (uint32_t) rows, offsets);
-            SKM_TRY(check_hip(hipGetLastError(), "key_bounds_kernel launch"));
-            lookup_grad_rows_kernel<T, O, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
-                (const T*) d_grad, grad_stride, index, offsets, rows, plan.most, scale, out, out_stride, accumulate, s);
-            SKM_TRY(check_hip(hipGetLastError(), "lookup_grad_rows_kernel launch"));
-            const uint64_t units = (uint64_t) plan.chunks * pieces;
-            const unsigned blocks = (unsigned) ((units + ROWS_THREADS / 64 - 1) / (ROWS_THREADS / 64));
-            lookup_grad_chunks_kernel<T, E><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
-                (const T*) d_grad, grad_stride, keys, index, offsets, (uint32_t) n, (uint32_t) rows, plan.most, parts, vectors, pieces,
-                plan.chunks);
-            SKM_TRY(check_hip(hipGetLastError(), "lookup_grad_chunks_kernel launch"));
-            lookup_grad_join_kernel<O, E><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
-                keys, offsets, (uint32_t) n, (uint32_t) rows, plan.most, parts, scale, out, out_stride, accumulate, vectors, pieces,
-                plan.chunks);
+            g.keys = (const uint32_t*) (scratch + plan.sort.at_keys[plan.sort.last()]);
+            g.index = (const uint32_t*) (scratch + plan.sort.at_index[plan.sort.last()]);
+            g.chunk = plan.chunk;
+            g.chunks = plan.chunks;
+            g.parts = (float*) (scratch + plan.at_parts);
+            const RowSplit s = split_rows(plan.chunks, g.vectors, GRAD_VECTORS);
+            constexpr uint64_t PER_BLOCK = ROWS_THREADS / 64;
+            const uint64_t chunk_blocks = (s.units + PER_BLOCK - 1) / PER_BLOCK;
+            const uint64_t fill_units = accumulate ? 0 : (rows + FILL_ROWS - 1) / FILL_ROWS;
+            const uint64_t blocks = chunk_blocks + (fill_units + PER_BLOCK - 1) / PER_BLOCK;
+            if (blocks > 0x7fffffffULL || (uint64_t) g.chunks * g.pieces > 0x7fffffffULL)
+                return set_error(SKM_ERR_INVALID, "skm_lookup_rows_grad: too many rows for one launch");
+            lookup_grad_kernel<T, O, E><<<(unsigned) blocks, ROWS_THREADS, 0, ctx->stream>>>(g, s, (uint32_t) chunk_blocks);
+            SKM_TRY(check_hip(hipGetLastError(), "lookup_grad_kernel launch"));
+            const uint32_t alone_blocks = (uint32_t) (((uint64_t) g.chunks * g.pieces + PER_BLOCK - 1) / PER_BLOCK);
+            const uint32_t long_blocks = (g.chunks + JOIN_ALONE - 1) / JOIN_ALONE * g.pieces;
+            lookup_grad_join_kernel<O, E><<<alone_blocks + long_blocks, ROWS_THREADS, 0, ctx->stream>>>(g, alone_blocks);
             return check_hip(hipGetLastError(), "lookup_grad_join_kernel launch");
         });
     };

@@ -24,24 +24,36 @@ import numpy as np
 
 from . import _capi
 
-_VALUES = {"float32": 0, "float16": 1, "bfloat16": 2}  # SKM_F32, SKM_F16, SKM_BF16
-_IDS = {"int32": 3, "uint32": 3, "int64": 4}  # SKM_U32 (a negative 32-bit id is a large one: no row), SKM_I64
-_WORDS = ("int32", "uint32")
 _SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "uint32": 4, "int64": 8, "int8": 1, "uint8": 1}
-
-_dtype_names = {}
 
 
 def _dtype_name(dtype):
     """"float32" for numpy's and torch's float32 alike."""
-    name = _dtype_names.get(dtype)
-    if name is None:
-        if isinstance(dtype, (np.dtype, type)):
-            name = np.dtype(dtype).name
-        else:
-            name = str(dtype).rsplit(".", 1)[-1]
-        _dtype_names[dtype] = name
-    return name
+    if isinstance(dtype, (np.dtype, type)):
+        return np.dtype(dtype).name
+    return str(dtype).rsplit(".", 1)[-1]
+
+
+class _Kinds(dict):
+    """dtype object -> code of the C interface, for the types that an argument may have; filled as dtypes come along."""
+
+    def __init__(self, codes):
+        super().__init__()
+        self.codes = codes
+
+    def __missing__(self, dtype):
+        name = _dtype_name(dtype)
+        if name not in self.codes:
+            raise TypeError(f"must be {' or '.join(self.codes)}, not {name}")
+        self[dtype] = self.codes[name]
+        return self[dtype]
+
+
+_VALUES = _Kinds({"float32": 0, "float16": 1, "bfloat16": 2})  # SKM_F32, SKM_F16, SKM_BF16
+_IDS = _Kinds({"int32": 3, "uint32": 3, "int64": 4})  # SKM_U32 (a negative 32-bit id is a large one: no row), SKM_I64
+_WORDS = _Kinds({"int32": 3, "uint32": 3})
+_STEPS = _Kinds({"int8": 5})
+_F32 = _Kinds({"float32": 0})
 
 
 class RowOperators:
@@ -65,12 +77,13 @@ class RowOperators:
         self.ctx = _capi.Context(device, stream) if ctx is None else ctx
         self.device = device
         self._lib = self.ctx.lib
+        self._handle = self.ctx.handle
 
     def close(self):
         """Releases the context, if it is the object's own."""
         if self._owned and self.ctx is not None:
             self.ctx.close()
-        self.ctx = None
+        self.ctx = self._handle = None  # a call after this is refused by the library: null context
 
     def __enter__(self):
         return self
@@ -89,59 +102,62 @@ class RowOperators:
         self.ctx.sync()
 
     # -- arguments ---------------------------------------------------------------------------------------------------
+    # A decoding step's calls are short: these checks are written for few attribute reads, not for few lines.
 
-    def _tensor(self, x, what, dtypes, ndim):
-        """(address, dtype name, shape, strides in elements) of a tensor on this device."""
-        if isinstance(x, _capi.DeviceArray):
-            shape, strides, address, step = x.shape, [], x.ptr, 1
-            for size in reversed(shape):
-                strides.insert(0, step)
-                step *= size
-        else:
-            try:
-                shape, strides, address = x.shape, x.stride(), x.data_ptr()
-            except AttributeError:
-                raise TypeError(f"{what} must be a device tensor, not {type(x).__name__}") from None
+    def _where(self, x, what):
+        """The address of a tensor on this device."""
+        try:
+            index = x.get_device()
+        except AttributeError:
             where = getattr(x, "device", None)
-            if where is not None:
-                kind = getattr(where, "type", "cuda")
-                if kind != "cuda" or where.index != self.device:
-                    raise ValueError(f"{what} is on {where}, not on device {self.device}")
-        name = _dtype_name(x.dtype)
-        if name not in dtypes:
-            raise TypeError(f"{what} must be {' or '.join(dtypes)}, not {name}")
-        if len(shape) != ndim:
-            raise ValueError(f"{what} must have {ndim} dimension{'s' if ndim > 1 else ''}, not {len(shape)}")
-        return address or None, name, shape, strides
+            index = self.device if where is None else where.index if getattr(where, "type", "cuda") == "cuda" else -1
+        if index != self.device:
+            raise ValueError(f"{what} is on {x.device}, not on device {self.device}")
+        return x.data_ptr() or None
 
-    def _matrix(self, x, what, dtypes):
-        """(address, dtype name, rows, columns, row stride): columns next to each other, rows any distance apart."""
-        address, name, (rows, columns), (row_stride, column_stride) = self._tensor(x, what, dtypes, 2)
-        if columns > 1 and column_stride != 1:
+    def _refuse(self, x, what, error):
+        """Says what is wrong with an argument whose attributes did not fit."""
+        for name in ("shape", "stride", "dtype", "data_ptr"):
+            if not hasattr(x, name):
+                raise TypeError(f"{what} must be a device tensor, not {type(x).__name__}") from None
+        if isinstance(error, TypeError):
+            raise TypeError(f"{what} {error}") from None
+        raise ValueError(f"{what} has {len(x.shape)} dimensions, which is not what it should have") from None
+
+    def _matrix(self, x, what, kinds):
+        """(address, type code, rows, columns, row stride): columns next to each other, rows any distance apart."""
+        try:
+            kind = kinds[x.dtype]
+            rows, columns = x.shape
+            row_stride, column_stride = x.stride()
+        except (AttributeError, TypeError, ValueError) as e:
+            self._refuse(x, what, e)
+        if column_stride != 1 and columns > 1:
             raise ValueError(f"{what} must have its columns next to each other")
-        if rows > 1:
-            if row_stride < columns:
+        if row_stride < columns:
+            if rows > 1:
                 raise ValueError(f"{what} has rows that overlap")
-        else:
             row_stride = columns
-        return address, name, rows, columns, row_stride
+        return self._where(x, what), kind, rows, columns, row_stride
 
-    def _dense(self, x, what, dtypes, shape):
-        """(address, dtype name) of a contiguous tensor of the given shape."""
-        address, name, has, strides = self._tensor(x, what, dtypes, len(shape))
-        if tuple(has) != shape:
-            raise ValueError(f"{what} must have shape {shape}, not {tuple(has)}")
-        step = 1
-        for size, stride in zip(reversed(shape), reversed(strides)):
-            if size > 1 and stride != step:
-                raise ValueError(f"{what} must be contiguous")
-            step *= size
-        return address, name
+    def _vector(self, x, what, kinds):
+        """(address, type code, length) of a contiguous vector."""
+        try:
+            kind = kinds[x.dtype]
+            (n,) = x.shape
+            (stride,) = x.stride()
+        except (AttributeError, TypeError, ValueError) as e:
+            self._refuse(x, what, e)
+        if stride != 1 and n > 1:
+            raise ValueError(f"{what} must be contiguous")
+        return self._where(x, what), kind, n
 
-    def _slots(self, slots):
-        address, _, (n, choices), _ = self._tensor(slots, "slots", _WORDS, 2)
-        self._dense(slots, "slots", _WORDS, (n, choices))
-        return address, n, choices
+    def _dense(self, x, what, kinds):
+        """(address, type code, rows, columns) of a contiguous matrix."""
+        at, kind, rows, columns, row_stride = self._matrix(x, what, kinds)
+        if row_stride != columns and rows > 1:
+            raise ValueError(f"{what} must be contiguous")
+        return at, kind, rows, columns
 
     def _scratch(self, scratch):
         if scratch is None:
@@ -149,16 +165,23 @@ class RowOperators:
         name = _dtype_name(scratch.dtype)
         if name not in _SIZES:
             raise TypeError(f"scratch cannot be of {name}")
-        address, _, (n,), (stride,) = self._tensor(scratch, "scratch", (name,), 1)
-        if n > 1 and stride != 1:
-            raise ValueError("scratch must be contiguous")
-        return address, n * _SIZES[name]
+        at, _, n = self._vector(scratch, "scratch", _Kinds({name: 0}))
+        return at, n * _SIZES[name]
 
     def _call(self, rc):
+        if rc == 0:
+            return
         if rc == _capi.SKM_ERR_INVALID:
             raise ValueError(self._lib.skm_last_error().decode())
-        if rc != 0:
-            _capi.check(rc)
+        _capi.check(rc)
+
+    @staticmethod
+    def _misfit(what, has, wants):
+        raise ValueError(f"{what} must have shape {wants}, not {has}")
+
+    @staticmethod
+    def _same_kind(what, has, wants):
+        raise TypeError(f"{what} must have the type of {wants}")
 
     # -- lookup ------------------------------------------------------------------------------------------------------
 
@@ -168,14 +191,14 @@ class RowOperators:
         table : (rows, d) float32, float16 or bfloat16;  ids : (n,) int32, uint32 or int64;  out : (n, d) of the table's type.
         """
         table_at, kind, rows, d, table_stride = self._matrix(table, "table", _VALUES)
-        ids_at, ids_kind, (n,), (ids_stride,) = self._tensor(ids, "ids", _IDS, 1)
-        out_at, _, out_rows, out_d, out_stride = self._matrix(out, "out", (kind,))
-        if n > 1 and ids_stride != 1:
-            raise ValueError("ids must be contiguous")
-        if (out_rows, out_d) != (n, d):
-            raise ValueError(f"out must have shape {(n, d)}, not {(out_rows, out_d)}")
-        self._call(self._lib.skm_lookup_rows(self.ctx.handle, table_at, _VALUES[kind], rows, d, table_stride, ids_at, _IDS[ids_kind], n,
-                                             scale, out_at, out_stride))
+        ids_at, ids_kind, n = self._vector(ids, "ids", _IDS)
+        out_at, out_kind, out_rows, out_d, out_stride = self._matrix(out, "out", _VALUES)
+        if out_kind != kind:
+            self._same_kind("out", out_kind, "table")
+        if out_rows != n or out_d != d:
+            self._misfit("out", (out_rows, out_d), (n, d))
+        self._call(self._lib.skm_lookup_rows(self._handle, table_at, kind, rows, d, table_stride, ids_at, ids_kind, n, scale, out_at,
+                                             out_stride))
         return out
 
     def lookup_grad(self, grad, ids, out, scale=1.0, accumulate=False, scratch=None):
@@ -186,18 +209,17 @@ class RowOperators:
         tensor of at least `lookup_grad_scratch` bytes, or None for the context's workspace (not under graph capture).
         """
         grad_at, kind, n, d, grad_stride = self._matrix(grad, "grad", _VALUES)
-        ids_at, ids_kind, (n_ids,), (ids_stride,) = self._tensor(ids, "ids", _IDS, 1)
-        out_at, out_kind, rows, out_d, out_stride = self._matrix(out, "out", (kind, "float32"))
-        if n > 1 and ids_stride != 1:
-            raise ValueError("ids must be contiguous")
+        ids_at, ids_kind, n_ids = self._vector(ids, "ids", _IDS)
+        out_at, out_kind, rows, out_d, out_stride = self._matrix(out, "out", _VALUES)
+        if out_kind != kind and out_kind != 0:
+            self._same_kind("out", out_kind, "grad, or float32")
         if n_ids != n:
-            raise ValueError(f"ids must have shape {(n,)}, not {(n_ids,)}")
+            self._misfit("ids", (n_ids,), (n,))
         if out_d != d:
-            raise ValueError(f"out must have {d} columns, not {out_d}")
+            self._misfit("out", (rows, out_d), (rows, d))
         scratch_at, scratch_bytes = self._scratch(scratch)
-        self._call(self._lib.skm_lookup_rows_grad(self.ctx.handle, grad_at, _VALUES[kind], grad_stride, ids_at, _IDS[ids_kind], n, rows, d,
-                                                  scale, out_at, _VALUES[out_kind], out_stride, 1 if accumulate else 0, scratch_at,
-                                                  scratch_bytes))
+        self._call(self._lib.skm_lookup_rows_grad(self._handle, grad_at, kind, grad_stride, ids_at, ids_kind, n, rows, d, scale, out_at,
+                                                  out_kind, out_stride, 1 if accumulate else 0, scratch_at, scratch_bytes))
         return out
 
     def lookup_grad_scratch(self, n, rows, d):
@@ -215,14 +237,20 @@ class RowOperators:
         place of every choice or -1 (0xffffffff); offsets (groups + 1,), the first place of every group and the number of places;
         order (n * k,), the choice t * k + j at every place, -1 behind the last one.  scratch: as in `lookup_grad`.
         """
-        choices_at, _, (n, k), _ = self._tensor(choices, "choices", _WORDS, 2)
-        self._dense(choices, "choices", _WORDS, (n, k))
-        slots_at, _ = self._dense(slots, "slots", _WORDS, (n, k))
-        offsets_at, _ = self._dense(offsets, "offsets", _WORDS, (groups + 1,))
-        order_at = None if order is None else self._dense(order, "order", _WORDS, (n * k,))[0]
+        choices_at, _, n, k = self._dense(choices, "choices", _WORDS)
+        slots_at, _, slots_n, slots_k = self._dense(slots, "slots", _WORDS)
+        offsets_at, _, n_offsets = self._vector(offsets, "offsets", _WORDS)
+        if slots_n != n or slots_k != k:
+            self._misfit("slots", (slots_n, slots_k), (n, k))
+        if n_offsets != groups + 1:
+            self._misfit("offsets", (n_offsets,), (groups + 1,))
+        order_at = None
+        if order is not None:
+            order_at, _, n_order = self._vector(order, "order", _WORDS)
+            if n_order != n * k:
+                self._misfit("order", (n_order,), (n * k,))
         scratch_at, scratch_bytes = self._scratch(scratch)
-        self._call(self._lib.skm_route(self.ctx.handle, choices_at, n, k, groups, slots_at, order_at, offsets_at, scratch_at,
-                                       scratch_bytes))
+        self._call(self._lib.skm_route(self._handle, choices_at, n, k, groups, slots_at, order_at, offsets_at, scratch_at, scratch_bytes))
         return slots, offsets
 
     def route_scratch(self, n, choices, groups):
@@ -237,12 +265,15 @@ class RowOperators:
         x : (n, d);  slots : (n, k);  out : (places, d) of x's type.
         """
         x_at, kind, n, d, x_stride = self._matrix(x, "x", _VALUES)
-        slots_at, slots_n, k = self._slots(slots)
-        out_at, _, out_rows, out_d, out_stride = self._matrix(out, "out", (kind,))
-        if slots_n != n or out_d != d:
-            raise ValueError(f"slots must have {n} rows and out {d} columns, not {slots_n} and {out_d}")
-        self._call(self._lib.skm_dispatch_rows(self.ctx.handle, x_at, _VALUES[kind], n, d, x_stride, slots_at, k, out_at, out_rows,
-                                               out_stride))
+        slots_at, _, slots_n, k = self._dense(slots, "slots", _WORDS)
+        out_at, out_kind, out_rows, out_d, out_stride = self._matrix(out, "out", _VALUES)
+        if out_kind != kind:
+            self._same_kind("out", out_kind, "x")
+        if slots_n != n:
+            self._misfit("slots", (slots_n, k), (n, k))
+        if out_d != d:
+            self._misfit("out", (out_rows, out_d), (out_rows, d))
+        self._call(self._lib.skm_dispatch_rows(self._handle, x_at, kind, n, d, x_stride, slots_at, k, out_at, out_rows, out_stride))
         return out
 
     def combine(self, rows, slots, out, weights=None):
@@ -251,16 +282,19 @@ class RowOperators:
         rows : (places, d);  slots : (n, k);  weights : (n, k) float32, float16 or bfloat16;  out : (n, d) of the rows' type.
         """
         rows_at, kind, n_rows, d, rows_stride = self._matrix(rows, "rows", _VALUES)
-        slots_at, n, k = self._slots(slots)
-        out_at, _, out_rows, out_d, out_stride = self._matrix(out, "out", (kind,))
-        if (out_rows, out_d) != (n, d):
-            raise ValueError(f"out must have shape {(n, d)}, not {(out_rows, out_d)}")
-        weights_at, weights_type = None, 0
+        slots_at, _, n, k = self._dense(slots, "slots", _WORDS)
+        out_at, out_kind, out_rows, out_d, out_stride = self._matrix(out, "out", _VALUES)
+        if out_kind != kind:
+            self._same_kind("out", out_kind, "rows")
+        if out_rows != n or out_d != d:
+            self._misfit("out", (out_rows, out_d), (n, d))
+        weights_at, weights_kind = None, 0
         if weights is not None:
-            weights_at, name = self._dense(weights, "weights", _VALUES, (n, k))
-            weights_type = _VALUES[name]
-        self._call(self._lib.skm_combine_rows(self.ctx.handle, rows_at, _VALUES[kind], n_rows, d, rows_stride, slots_at, n, k, weights_at,
-                                              weights_type, out_at, out_stride))
+            weights_at, weights_kind, weights_n, weights_k = self._dense(weights, "weights", _VALUES)
+            if weights_n != n or weights_k != k:
+                self._misfit("weights", (weights_n, weights_k), (n, k))
+        self._call(self._lib.skm_combine_rows(self._handle, rows_at, kind, n_rows, d, rows_stride, slots_at, n, k, weights_at, weights_kind,
+                                              out_at, out_stride))
         return out
 
     def combine_grad(self, grad, rows, slots, weights, grad_rows, grad_weights):
@@ -270,32 +304,39 @@ class RowOperators:
         be None, and rows where grad_weights is; weights None stands for ones (grad_weights is then of any value type).
         """
         grad_at, kind, n, d, grad_stride = self._matrix(grad, "grad", _VALUES)
-        slots_at, slots_n, k = self._slots(slots)
+        slots_at, _, slots_n, k = self._dense(slots, "slots", _WORDS)
         if slots_n != n:
-            raise ValueError(f"slots must have {n} rows, not {slots_n}")
+            self._misfit("slots", (slots_n, k), (n, k))
         rows_at, rows_stride, n_rows, out_at, out_stride = None, d, None, None, d
         if rows is not None:
-            rows_at, _, n_rows, rows_d, rows_stride = self._matrix(rows, "rows", (kind,))
+            rows_at, rows_kind, n_rows, rows_d, rows_stride = self._matrix(rows, "rows", _VALUES)
+            if rows_kind != kind:
+                self._same_kind("rows", rows_kind, "grad")
             if rows_d != d:
-                raise ValueError(f"rows must have {d} columns, not {rows_d}")
+                self._misfit("rows", (n_rows, rows_d), (n_rows, d))
         elif grad_weights is not None:
             raise ValueError("grad_weights needs the rows")
         if grad_rows is not None:
-            out_at, _, out_rows, out_d, out_stride = self._matrix(grad_rows, "grad_rows", (kind,))
+            out_at, out_kind, out_rows, out_d, out_stride = self._matrix(grad_rows, "grad_rows", _VALUES)
+            if out_kind != kind:
+                self._same_kind("grad_rows", out_kind, "grad")
             if out_d != d or n_rows not in (None, out_rows):
-                raise ValueError("grad_rows must have the shape of rows")
+                self._misfit("grad_rows", (out_rows, out_d), (out_rows if n_rows is None else n_rows, d))
             n_rows = out_rows
-        weights_at, weights_type, grad_weights_at = None, 0, None
+        weights_at, weights_kind, grad_weights_at = None, 0, None
         if weights is not None:
-            weights_at, name = self._dense(weights, "weights", _VALUES, (n, k))
-            weights_type = _VALUES[name]
+            weights_at, weights_kind, weights_n, weights_k = self._dense(weights, "weights", _VALUES)
+            if weights_n != n or weights_k != k:
+                self._misfit("weights", (weights_n, weights_k), (n, k))
         if grad_weights is not None:
-            kinds = _VALUES if weights is None else (name,)
-            grad_weights_at, name = self._dense(grad_weights, "grad_weights", kinds, (n, k))
-            weights_type = _VALUES[name]
-        self._call(self._lib.skm_combine_rows_grad(self.ctx.handle, grad_at, _VALUES[kind], n, d, grad_stride, rows_at, n_rows or 0,
-                                                   rows_stride, slots_at, k, weights_at, weights_type, out_at, out_stride,
-                                                   grad_weights_at))
+            grad_weights_at, out_kind, weights_n, weights_k = self._dense(grad_weights, "grad_weights", _VALUES)
+            if weights is not None and out_kind != weights_kind:
+                self._same_kind("grad_weights", out_kind, "weights")
+            if weights_n != n or weights_k != k:
+                self._misfit("grad_weights", (weights_n, weights_k), (n, k))
+            weights_kind = out_kind
+        self._call(self._lib.skm_combine_rows_grad(self._handle, grad_at, kind, n, d, grad_stride, rows_at, n_rows or 0, rows_stride,
+                                                   slots_at, k, weights_at, weights_kind, out_at, out_stride, grad_weights_at))
         return grad_rows, grad_weights
 
     # -- 8-bit rows --------------------------------------------------------------------------------------------------
@@ -306,11 +347,13 @@ class RowOperators:
         x : (n, d);  q : (n, d) int8;  scales : (n,) float32.  A row with an infinity or NaN gets scale NaN.
         """
         x_at, kind, n, d, x_stride = self._matrix(x, "x", _VALUES)
-        q_at, _, q_n, q_d, q_stride = self._matrix(q, "q", ("int8",))
-        if (q_n, q_d) != (n, d):
-            raise ValueError(f"q must have shape {(n, d)}, not {(q_n, q_d)}")
-        scales_at, _ = self._dense(scales, "scales", ("float32",), (n,))
-        self._call(self._lib.skm_quantize_rows(self.ctx.handle, x_at, _VALUES[kind], n, d, x_stride, q_at, q_stride, scales_at))
+        q_at, _, q_n, q_d, q_stride = self._matrix(q, "q", _STEPS)
+        scales_at, _, n_scales = self._vector(scales, "scales", _F32)
+        if q_n != n or q_d != d:
+            self._misfit("q", (q_n, q_d), (n, d))
+        if n_scales != n:
+            self._misfit("scales", (n_scales,), (n,))
+        self._call(self._lib.skm_quantize_rows(self._handle, x_at, kind, n, d, x_stride, q_at, q_stride, scales_at))
         return q, scales
 
     def product(self, a, a_scales, b, b_scales, out, bias=None, offsets=None):
@@ -320,29 +363,48 @@ class RowOperators:
         as `route` makes them, b is (groups, n, k) and b_scales and bias (groups, n): the rows [offsets[g], offsets[g + 1]) are
         multiplied with b[g], and rows of out that are in no group stay as they are.
         """
-        a_at, _, m, k, a_stride = self._matrix(a, "a", ("int8",))
+        a_at, _, m, k, a_stride = self._matrix(a, "a", _STEPS)
         out_at, out_kind, out_m, n, out_stride = self._matrix(out, "out", _VALUES)
+        a_scales_at, _, n_scales = self._vector(a_scales, "a_scales", _F32)
+        if n_scales != m:
+            self._misfit("a_scales", (n_scales,), (m,))
+        bias_at = offsets_at = None
+        groups, group_stride = 1, 0
         if offsets is None:
-            groups, group_stride, offsets_at = 1, 0, None
-            b_at, _, b_n, b_k, b_stride = self._matrix(b, "b", ("int8",))
-            per_column = (n,)
+            b_at, _, b_n, b_k, b_stride = self._matrix(b, "b", _STEPS)
+            b_scales_at, _, scales_n = self._vector(b_scales, "b_scales", _F32)
+            if bias is not None:
+                bias_at, _, bias_n = self._vector(bias, "bias", _F32)
+                if bias_n != n:
+                    self._misfit("bias", (bias_n,), (n,))
         else:
-            b_at, _, (groups, b_n, b_k), (group_stride, b_stride, column_stride) = self._tensor(b, "b", ("int8",), 3)
-            if b_k > 1 and column_stride != 1:
+            try:
+                _STEPS[b.dtype]
+                groups, b_n, b_k = b.shape
+                group_stride, b_stride, column_stride = b.stride()
+            except (AttributeError, TypeError, ValueError) as e:
+                self._refuse(b, "b", e)
+            b_at = self._where(b, "b")
+            if column_stride != 1 and b_k > 1:
                 raise ValueError("b must have its columns next to each other")
             if b_n == 1:
-                b_stride = b_k
+                b_stride = max(b_stride, b_k)
+            if b_stride < b_k or groups > 1 and group_stride < (b_n - 1) * b_stride + b_k:
+                raise ValueError("b has rows that overlap")
             if groups == 1:
                 group_stride = 0
-            if b_n > 1 and b_stride < b_k or groups > 1 and group_stride < (b_n - 1) * b_stride + b_k:
-                raise ValueError("b has rows that overlap")
-            offsets_at, _ = self._dense(offsets, "offsets", _WORDS, (groups + 1,))
-            per_column = (groups, n)
-        if out_m != m or b_n != n or b_k != k:
-            raise ValueError(f"a {(m, k)}, b {(b_n, b_k)} and out {(out_m, n)} do not fit together")
-        a_scales_at, _ = self._dense(a_scales, "a_scales", ("float32",), (m,))
-        b_scales_at, _ = self._dense(b_scales, "b_scales", ("float32",), per_column)
-        bias_at = None if bias is None else self._dense(bias, "bias", ("float32",), per_column)[0]
-        self._call(self._lib.skm_product_i8(self.ctx.handle, a_at, m, a_stride, a_scales_at, b_at, n, k, b_stride, b_scales_at, bias_at,
-                                            groups, group_stride, offsets_at, out_at, _VALUES[out_kind], out_stride))
+            offsets_at, _, n_offsets = self._vector(offsets, "offsets", _WORDS)
+            if n_offsets != groups + 1:
+                self._misfit("offsets", (n_offsets,), (groups + 1,))
+            b_scales_at, _, scales_groups, scales_n = self._dense(b_scales, "b_scales", _F32)
+            if scales_groups != groups:
+                self._misfit("b_scales", (scales_groups, scales_n), (groups, n))
+            if bias is not None:
+                bias_at, _, bias_groups, bias_n = self._dense(bias, "bias", _F32)
+                if bias_groups != groups or bias_n != n:
+                    self._misfit("bias", (bias_groups, bias_n), (groups, n))
+        if out_m != m or b_n != n or b_k != k or scales_n != n:
+            raise ValueError(f"a {(m, k)}, b {(b_n, b_k)}, b_scales of {scales_n} and out {(out_m, n)} do not fit together")
+        self._call(self._lib.skm_product_i8(self._handle, a_at, m, a_stride, a_scales_at, b_at, n, k, b_stride, b_scales_at, bias_at, groups,
+                                            group_stride, offsets_at, out_at, out_kind, out_stride))
         return out

@@ -108,6 +108,8 @@ BAD = {
     "product groups of other offsets": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8)), T((2, 5)), T((3, 5)), offsets=I((2,))),
     "product groups that overlap": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8), stride=(8, 8, 1)), T((2, 5)), T((3, 5)),
                                                        offsets=I((3,))),
+    "product with rows that overlap": lambda o: o.product(q8((3, 8)), T((3,)), q8((1, 5, 8), stride=(40, 4, 1)), T((1, 5)), T((3, 5)),
+                                                          offsets=I((2,))),
     "product with a bias for all groups": lambda o: o.product(q8((3, 8)), T((3,)), q8((2, 5, 8)), T((2, 5)), T((3, 5)), bias=T((5,)),
                                                               offsets=I((3,))),
 }
