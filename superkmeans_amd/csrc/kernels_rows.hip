@@ -36,36 +36,41 @@ __device__ __forceinline__ uint64_t id_at(const void* ids, const int ids_type, c
     return ids_type == SKM_I64 ? reinterpret_cast<const uint64_t*>(ids)[i] : (uint64_t) reinterpret_cast<const uint32_t*>(ids)[i];
 }
 
-// out[t] = scale * table[id_t], a row of zeros where the id is no row.  A lane requests UNROLL vectors of its row before
-// it stores the first.
-template <class T, int E>
+// out[t] = scale * table[id_t], a row of zeros where the id is no row.  A wavefront takes TOKENS rows at a time and requests all
+// their ids, then UNROLL vectors per lane of all the rows, before it stores the first: with one row at a time the wavefronts
+// that a compute unit holds do not have enough bytes on their way.
+template <class T, int E, int TOKENS>
 __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
     const T* __restrict__ table, const size_t rows, const size_t table_stride, const void* __restrict__ ids, const int ids_type,
     const size_t n, const float scale, T* __restrict__ out, const size_t out_stride, const RowSplit s
 ) {
-    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes;
+    const uint32_t lane = threadIdx.x & 63, in_row = lane & (s.lanes - 1), row_of_wave = lane / s.lanes, rows_of_wave = 64 / s.lanes;
     const uint64_t step = (uint64_t) gridDim.x * (ROWS_THREADS / 64);
     for (uint64_t u = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + (threadIdx.x >> 6); u < s.units; u += step) {
-        const size_t t = (size_t) (u / s.pieces) * (64 / s.lanes) + row_of_wave;
-        if (t >= n) continue;
+        const size_t t = (size_t) (u / s.pieces) * (TOKENS * rows_of_wave) + row_of_wave;
         const uint32_t first = (uint32_t) (u % s.pieces) * s.lanes * UNROLL + in_row;
-        const uint64_t id = id_at(ids, ids_type, t);
-        const bool there = id < rows;
-        const T* from = table + (there ? id : 0) * table_stride;
-        T* to = out + t * out_stride;
-        vec_of<T, E> v[UNROLL];
+        uint64_t id[TOKENS];
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors && there) v[i] = load_vec<T, E>(from + (size_t) at * E);
-        }
+        for (int q = 0; q < TOKENS; ++q) id[q] = t + q * rows_of_wave < n ? id_at(ids, ids_type, t + q * rows_of_wave) : rows;
+        vec_of<T, E> v[TOKENS][UNROLL];
 #pragma unroll
-        for (int i = 0; i < UNROLL; ++i) {
-            const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors) {
-                vec_of<T, E> r = {};
-                if (there) r = scale == 1.0f ? v[i] : narrow<T, E>(widen<E>(v[i]) * scale);
-                store_vec<T, E>(to + (size_t) at * E, r);
+        for (int q = 0; q < TOKENS; ++q)
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i) {
+                const uint32_t at = first + i * s.lanes;
+                if (at < s.vectors && id[q] < rows) v[q][i] = load_vec<T, E>(table + id[q] * table_stride + (size_t) at * E);
+                else v[q][i] = vec_of<T, E>{};
+            }
+#pragma unroll
+        for (int q = 0; q < TOKENS; ++q) {
+            if (t + q * rows_of_wave >= n) break;
+#pragma unroll
+            for (int i = 0; i < UNROLL; ++i) {
+                const uint32_t at = first + i * s.lanes;
+                if (at < s.vectors) {
+                    const vec_of<T, E> r = scale == 1.0f || id[q] >= rows ? v[q][i] : narrow<T, E>(widen<E>(v[q][i]) * scale);
+                    store_vec_once<T, E>(out + (t + q * rows_of_wave) * out_stride + (size_t) at * E, r);
+                }
             }
         }
     }
@@ -87,7 +92,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
             const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors) v[i] = load_vec<T, E>(x + t * x_stride + (size_t) at * E);
+            if (at < s.vectors) v[i] = load_vec_once<T, E>(x + t * x_stride + (size_t) at * E);
         }
         for (uint32_t j = 0; j < choices; ++j) {
             const uint32_t slot = slots[t * choices + j];
@@ -95,7 +100,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i) {
                 const uint32_t at = first + i * s.lanes;
-                if (at < s.vectors) store_vec<T, E>(out + (size_t) slot * out_stride + (size_t) at * E, v[i]);
+                if (at < s.vectors) store_vec_once<T, E>(out + (size_t) slot * out_stride + (size_t) at * E, v[i]);
             }
         }
     }
@@ -112,8 +117,8 @@ __device__ __forceinline__ void put_weight(void* weights, const int type, const 
     else reinterpret_cast<__bf16*>(weights)[i] = (__bf16) v;
 }
 
-constexpr int COMBINE_UNROLL = 2;  // vectors per lane
-constexpr int COMBINE_AHEAD = 4;   // choices whose rows are requested together
+constexpr int COMBINE_UNROLL = 4;  // vectors per lane
+constexpr int COMBINE_AHEAD = 2;   // choices whose rows are requested together
 
 // out[t] = sum_j w[t][j] * rows[slot[t][j]], j ascending, in fp32.
 template <class T, int E>
@@ -145,7 +150,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
                 for (int i = 0; i < COMBINE_UNROLL; ++i) {
                     const uint32_t at = first + i * s.lanes;
                     if (slot[j] < n_rows && at < s.vectors)
-                        v[j][i] = load_vec<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                        v[j][i] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
                 }
 #pragma unroll
             for (int j = 0; j < COMBINE_AHEAD; ++j)
@@ -156,16 +161,14 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
 #pragma unroll
         for (int i = 0; i < COMBINE_UNROLL; ++i) {
             const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors) store_vec<T, E>(out + t * out_stride + (size_t) at * E, narrow<T, E>(sum[i]));
+            if (at < s.vectors) store_vec_once<T, E>(out + t * out_stride + (size_t) at * E, narrow<T, E>(sum[i]));
         }
     }
 }
 
-constexpr int GRAD_CHOICES = 8;  // choices whose products are summed in one walk over the row
-
 // grad_rows[slot[t][j]] = w[t][j] * grad[t] and grad_w[t][j] = <grad[t], rows[slot[t][j]]>: one walk over the token's row
 // for each GRAD_CHOICES choices, WAVES wavefronts per token.
-template <class T, int E, int WAVES>
+template <class T, int E, int WAVES, int GRAD_CHOICES>
 __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
     const T* __restrict__ grad, const size_t n, const uint32_t vectors, const size_t grad_stride, const T* __restrict__ rows,
     const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const uint32_t choices,
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
                     if (grad_weights) {
 #pragma unroll
                         for (int j = 0; j < GRAD_CHOICES; ++j)
-                            if (slot[j] < n_rows) y[j] = load_vec<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                            if (slot[j] < n_rows) y[j] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
                     }
 #pragma unroll
                     for (int j = 0; j < GRAD_CHOICES; ++j) {
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
                             dot[j] += sum;
                         }
                         if (grad_rows)
-                            store_vec<T, E>(grad_rows + (size_t) slot[j] * grad_rows_stride + (size_t) at * E, narrow<T, E>(g * w[j]));
+                            store_vec_once<T, E>(grad_rows + (size_t) slot[j] * grad_rows_stride + (size_t) at * E, narrow<T, E>(g * w[j]));
                     }
                 }
             }
@@ -269,10 +272,16 @@ int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, si
         using T = decltype(sample);
         return for_width<T>(width, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const RowSplit s = split_rows(n, d / E, UNROLL);
-            lookup_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
-                (const T*) d_table, rows, table_stride, d_ids, ids_type, n, scale, (T*) d_out, out_stride, s);
-            return check_hip(hipGetLastError(), "lookup_rows_kernel launch");
+            const auto launch = [&](auto tokens) {
+                constexpr int TOKENS = decltype(tokens)::value;
+                const RowSplit s = split_rows((n + TOKENS - 1) / TOKENS, d / E, UNROLL);
+                lookup_rows_kernel<T, E, TOKENS><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
+                    (const T*) d_table, rows, table_stride, d_ids, ids_type, n, scale, (T*) d_out, out_stride, s);
+                return check_hip(hipGetLastError(), "lookup_rows_kernel launch");
+            };
+            // several rows to a wavefront once there are wavefronts for the whole chip all the same (32 on each compute unit)
+            if (split_rows(n, d / E, UNROLL).units >= 4 * 8192) return launch(std::integral_constant<int, 4>{});
+            return launch(std::integral_constant<int, 1>{});
         });
     });
 }
@@ -371,17 +380,22 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
         return for_width<T>(width, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
             const uint32_t vectors = (uint32_t) (d / E);
-            const auto launch = [&](auto waves) {
+            const auto launch = [&](auto waves, auto together) {
                 constexpr int WAVES = decltype(waves)::value;
                 const size_t turns = (n + ROWS_THREADS / 64 / WAVES - 1) / (ROWS_THREADS / 64 / WAVES);
                 const unsigned blocks = (unsigned) std::min<uint64_t>(ROWS_MAX_BLOCKS, turns);
-                combine_rows_grad_kernel<T, E, WAVES><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
+                combine_rows_grad_kernel<T, E, WAVES, decltype(together)::value><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
                     (const T*) d_grad, n, vectors, grad_stride, (const T*) d_rows, n_rows, rows_stride, d_slots, (uint32_t) choices,
                     d_weights, weights_type, (T*) d_grad_rows, grad_rows_stride, d_grad_weights);
                 return check_hip(hipGetLastError(), "combine_rows_grad_kernel launch");
             };
-            if (vectors > 64) return launch(std::integral_constant<int, 4>{});
-            return launch(std::integral_constant<int, 1>{});
+            const auto launch_waves = [&](auto waves) {
+                if (choices <= 2) return launch(waves, std::integral_constant<int, 2>{});
+                if (choices <= 4) return launch(waves, std::integral_constant<int, 4>{});
+                return launch(waves, std::integral_constant<int, 8>{});
+            };
+            if (vectors > 64) return launch_waves(std::integral_constant<int, 4>{});
+            return launch_waves(std::integral_constant<int, 1>{});
         });
     });
 }

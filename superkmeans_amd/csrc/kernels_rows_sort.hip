@@ -338,7 +338,7 @@ template <class O, int E>
 __device__ __forceinline__ void put_sum(O* to, const vec_of<float, E> sum, const float scale, const bool accumulate) {
     vec_of<float, E> r = sum * scale;
     if (accumulate) r += widen<E>(load_vec<O, E>(to));
-    store_vec<O, E>(to, narrow<O, E>(r));
+    store_vec_once<O, E>(to, narrow<O, E>(r));
 }
 
 struct GradArgs {
@@ -347,7 +347,7 @@ struct GradArgs {
     void* out;
     size_t out_stride;
     float scale;
-    int accumulate;
+    bool accumulate;
     uint32_t n, rows, vectors, pieces;  // vectors per row; pieces of 64 vectors
     // sorted tokens: their keys and positions, in chunks of `chunk`, and the chunks' sums of rows that go past them
     const uint32_t *keys, *index;
@@ -438,7 +438,7 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit
     }
     for (unsigned long long left = __ballot(empty); left; left &= left - 1) {
         O* out = reinterpret_cast<O*>(g.out) + (size_t) (unit * FILL_ROWS + (uint32_t) __builtin_ctzll(left)) * g.out_stride;
-        for (uint32_t at = lane; at < g.vectors; at += 64) store_vec<O, E>(out + (size_t) at * E, vec_of<O, E>{});
+        for (uint32_t at = lane; at < g.vectors; at += 64) store_vec_once<O, E>(out + (size_t) at * E, vec_of<O, E>{});
     }
 }
 
@@ -641,7 +641,7 @@ struct GradPlan {
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
         // The additions of a chunk, and of a row's chunks, are chains: longer chunks for more tokens keep the second short
         // where many tokens are on one row.
-        chunk = n <= (size_t(1) << 17) ? 32 : n <= (size_t(1) << 20) ? 128 : 256;
+        chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 128 : 256;
         chunks = (uint32_t) ((n + chunk - 1) / chunk);
         at_parts = sort.bytes;
         bytes = at_parts + aligned((size_t) chunks * 2 * d * 4);
