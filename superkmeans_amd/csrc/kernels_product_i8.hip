@@ -17,51 +17,99 @@ typedef int intx16 __attribute__((ext_vector_type(16)));
 // Quantisation
 // ---------------------------------------------------------------------------------------------
 
-// The whole number nearest to 127 x / most, ties to even.  The fp32 product is at most 2 units of its last place off
-// (3e-5 at 127), so that the choice between two numbers can only be wrong next to the border between them; there the
-// quotient is taken in fp64, where 127 x is exact and a quotient of two fp32 numbers cannot round onto a border.
-__device__ __forceinline__ int nearest_step(const float x, const float most, const float inverse) {
-    const float t = x * inverse;
-    const float r = rintf(t);
-    if (fabsf(t - r) < 0.4999f) return (int) r;
-    return (int) rint((double) x * 127.0 / (double) most);
+// The whole numbers nearest to 127 x / most, ties to even, as bytes.  The fp32 product of x and the rounded 127 / most is at most
+// 127 * 2^-23 = 1.6e-5 off, so that the choice between two numbers can only be wrong that near to the border between them; there
+// the quotient is taken in fp64, where 127 x is exact and a quotient of two fp32 numbers cannot round onto a border.  Adding
+// 1.5 * 2^23 rounds an fp32 number of that size to a whole one, whose last byte is the step.
+template <int E>
+__device__ __forceinline__ vec_of<int8_t, E> nearest_steps(const vec_of<float, E> x, const float most, const float inverse) {
+    uint32_t step[E];
+    bool border = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float t = x[e] * inverse, shifted = t + 12582912.0f;
+        border |= !(fabsf(t - (shifted - 12582912.0f)) < 0.49998f);
+        step[e] = __float_as_uint(shifted);
+    }
+    if (border)
+#pragma unroll
+        for (int e = 0; e < E; ++e) step[e] = (uint32_t) (int) rint((double) x[e] * 127.0 / (double) most);
+    if constexpr (E % 4 == 0) {
+        vec_of<uint32_t, E / 4> words;
+#pragma unroll
+        for (int w = 0; w < E / 4; ++w) {
+            const uint32_t low = __builtin_amdgcn_perm(step[4 * w + 1], step[4 * w], 0x0c0c0400u);
+            const uint32_t high = __builtin_amdgcn_perm(step[4 * w + 3], step[4 * w + 2], 0x0c0c0400u);
+            words[w] = __builtin_amdgcn_perm(high, low, 0x05040100u);
+        }
+        return __builtin_bit_cast(vec_of<int8_t, E>, words);
+    } else {
+        vec_of<int8_t, E> r;
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[e] = (int8_t) step[e];
+        return r;
+    }
 }
 
+// Largest magnitudes, element by element, as the numbers' bits without the sign: ordered like the numbers, infinities and NaN
+// above all.
+template <class T, int E>
+using bits_of = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> __attribute__((ext_vector_type(E)));
+
+// WAVES wavefronts to a row.  A row of up to 64 WAVES HELD vectors is read once and held in registers; of a longer one what is
+// past that is read twice.
 constexpr int QUANTIZE_THREADS = 256;
 
-template <class T, int E>
+template <class T, int E, int WAVES, int HELD>
 __global__ __launch_bounds__(QUANTIZE_THREADS) void quantize_rows_kernel(
     const T* __restrict__ x, const size_t n, const uint32_t vectors, const size_t x_stride, int8_t* __restrict__ q,
     const size_t q_stride, float* __restrict__ scales
 ) {
+    constexpr int ROWS = QUANTIZE_THREADS / 64 / WAVES, LANES = 64 * WAVES;  // ROWS per workgroup
     __shared__ uint32_t wave_most[QUANTIZE_THREADS / 64];
-    for (size_t t = blockIdx.x; t < n; t += gridDim.x) {
+    const uint32_t in_row = threadIdx.x % LANES;
+    const size_t turns = (n + ROWS - 1) / ROWS;  // the same for every thread, which all meet at the barriers
+    for (size_t turn = blockIdx.x; turn < turns; turn += gridDim.x) {
+        const size_t t = turn * ROWS + threadIdx.x / LANES;
         const T* row = x + t * x_stride;
-        uint32_t most = 0;  // bits of the largest magnitude: ordered like the numbers, infinities and NaN above all
-        for (uint32_t at = threadIdx.x; at < vectors; at += QUANTIZE_THREADS) {
-            const vec_of<float, E> v = widen<E>(load_vec<T, E>(row + (size_t) at * E));
+        const uint32_t mine = t < n ? vectors : 0;
+        bits_of<T, E> largest = 0;
+        const auto look = [&](const vec_of<T, E> v) {
+            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(bits_of<T, E>, v) & (bits_of<T, E>) (sizeof(T) == 2 ? 0x7fff : 0x7fffffff));
+        };
+        vec_of<T, E> held[HELD];
 #pragma unroll
-            for (int e = 0; e < E; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-        }
+        for (int i = 0; i < HELD; ++i)
+            if (in_row + i * LANES < mine) held[i] = load_vec<T, E>(row + (size_t) (in_row + i * LANES) * E);
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (in_row + i * LANES < mine) look(held[i]);
+        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) look(load_vec<T, E>(row + (size_t) at * E));
+        auto one = largest[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) one = one > largest[e] ? one : largest[e];
+        uint32_t most = __float_as_uint((float) __builtin_bit_cast(T, one));
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) most = max(most, (uint32_t) __shfl_xor(most, off));
-        if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
-        __syncthreads();
+        if (WAVES > 1) {
+            __syncthreads();  // the row before has been looked at
+            if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < QUANTIZE_THREADS / 64; ++w) most = max(most, wave_most[w]);
-        __syncthreads();
+            for (int w = 0; w < WAVES; ++w) most = max(most, wave_most[threadIdx.x / LANES * WAVES + w]);
+        }
         const bool usable = most != 0 && most < 0x7f800000u;
         const float m = __uint_as_float(most);
         const float inverse = m > 1e-30f ? 127.0f / m : __builtin_nanf("");  // NaN sends every element through fp64
-        if (threadIdx.x == 0) scales[t] = most < 0x7f800000u ? m / 127.0f : __builtin_nanf("");
-        for (uint32_t at = threadIdx.x; at < vectors; at += QUANTIZE_THREADS) {
-            const vec_of<float, E> v = widen<E>(load_vec<T, E>(row + (size_t) at * E));
-            vec_of<int8_t, E> r = {};
-            if (usable)
-#pragma unroll
-                for (int e = 0; e < E; ++e) r[e] = (int8_t) nearest_step(v[e], m, inverse);
+        if (in_row == 0 && t < n) scales[t] = most < 0x7f800000u ? m / 127.0f : __builtin_nanf("");
+        const auto put = [&](const uint32_t at, const vec_of<T, E> v) {
+            const vec_of<int8_t, E> r = usable ? nearest_steps<E>(widen<E>(v), m, inverse) : vec_of<int8_t, E>{};
             *reinterpret_cast<vec_of<int8_t, E>*>(q + t * q_stride + (size_t) at * E) = r;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (in_row + i * LANES < mine) put(in_row + i * LANES, held[i]);
+        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) put(at, load_vec<T, E>(row + (size_t) at * E));
     }
 }
 
@@ -120,11 +168,8 @@ __device__ __forceinline__ RowTile find_rows(const ProductArgs& p, const uint32_
     return {0, 0, 0};
 }
 
-// 16 bytes of a row.  Rows that are not aligned to 16 bytes are read with the same instruction, which takes any address;
-// only the compiler has to be told.
-template <bool ALIGNED>
+// 16 bytes of a row, at any address: the load instruction takes them unaligned too, only the compiler has to be told.
 __device__ __forceinline__ intx4 load16(const int8_t* p) {
-    if constexpr (ALIGNED) return *reinterpret_cast<const intx4*>(p);
     intx4 v;
     __builtin_memcpy(&v, p, 16);
     return v;
@@ -166,7 +211,7 @@ __device__ __forceinline__ intx4 load16_short(const int8_t* row, const int k, co
 // their 32-bit sums are added through LDS (exact, so the split does not show).  With a row or a few per matrix every
 // byte of the weights is read once and used at once, so nothing is gained by LDS; what counts is how many bytes are on their
 // way: each wavefront requests AHEAD steps of 64 columns before it uses the first.
-template <class O, int RT, int NB, int WAVES, int AHEAD, bool ALIGNED>
+template <class O, int RT, int NB, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs p, const uint32_t tiles_n) {
     constexpr int TM = 16 * RT, TN = 16 * NB;
     __shared__ int part[WAVES][TM][TN + 4];
@@ -191,41 +236,46 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const Prod
             for (int i = 0; i < RT; ++i) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[j][i], 0, 0, 0);
     };
     uint32_t s = from;
-    if (s + AHEAD <= full) {
-        intx4 x[AHEAD][RT], w[AHEAD][NB];
-        const auto request = [&](const int q, const uint32_t step) {
+    intx4 x[AHEAD][RT], w[AHEAD][NB];
+    const auto request = [&](const int q, const uint32_t step) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) w[q][j] = load16<ALIGNED>(b[j] + (size_t) step * 64);
+        for (int j = 0; j < NB; ++j) w[q][j] = load16(b[j] + (size_t) step * 64);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) x[q][i] = load16<ALIGNED>(a[i] + (size_t) step * 64);
-        };
+        for (int i = 0; i < RT; ++i) x[q][i] = load16(a[i] + (size_t) step * 64);
+    };
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q) request(q, s + q);
-        for (; s + 2 * AHEAD <= full; s += AHEAD)
+    for (int q = 0; q < AHEAD; ++q)
+        if (s + q < full) request(q, s + q);
+    for (; s + 2 * AHEAD <= full; s += AHEAD)
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q) {
-                multiply(x[q], w[q]);
-                request(q, s + AHEAD + q);
-            }
+        for (int q = 0; q < AHEAD; ++q) {
+            multiply(x[q], w[q]);
+            request(q, s + AHEAD + q);
+        }
+    // up to 2 AHEAD - 1 steps are left, the first AHEAD of them requested
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q) multiply(x[q], w[q]);
-        s += AHEAD;
-    }
-    for (; s < to; ++s) {
-        intx4 x[RT], w[NB];
-        const int skip = (lane >> 4) * 16, k = (int) (s * 64) + skip;
+    for (int q = 0; q < AHEAD; ++q)
+        if (s + q < full) {
+            multiply(x[q], w[q]);
+            if (s + AHEAD + q < full) request(q, s + AHEAD + q);
+        }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q)
+        if (s + AHEAD + q < full) multiply(x[q], w[q]);
+    if (from < to && full < to) {  // the columns' end
+        const int skip = (lane >> 4) * 16, k = (int) (full * 64) + skip;
         if (p.k >= 16) {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) w[j] = load16_end(b[j] - skip, k, (int) p.k);
+            for (int j = 0; j < NB; ++j) w[0][j] = load16_end(b[j] - skip, k, (int) p.k);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) x[i] = load16_end(a[i] - skip, k, (int) p.k);
+            for (int i = 0; i < RT; ++i) x[0][i] = load16_end(a[i] - skip, k, (int) p.k);
         } else {
 #pragma unroll
-            for (int j = 0; j < NB; ++j) w[j] = load16_short(b[j] - skip, k, (int) p.k);
+            for (int j = 0; j < NB; ++j) w[0][j] = load16_short(b[j] - skip, k, (int) p.k);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) x[i] = load16_short(a[i] - skip, k, (int) p.k);
+            for (int i = 0; i < RT; ++i) x[0][i] = load16_short(a[i] - skip, k, (int) p.k);
         }
-        multiply(x, w);
+        multiply(x[0], w[0]);
     }
     // block (j, i): lane l holds the columns 4 (l / 16) .. + 3 of the result's row l % 16
 #pragma unroll
@@ -275,7 +325,7 @@ struct TileMap {
     }
 };
 
-template <class O, int FM, int FN, bool ALIGNED>
+template <class O, int FM, int FN>
 __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(const ProductArgs p, const TileMap map) {
     constexpr int TM = 64 * FM, TN = 64 * FN, NLA = TM / 32, NLB = TN / 32;
     constexpr uint32_t STAGE = (TM + TN) * STAGE_K;
@@ -302,9 +352,9 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     const auto request = [&](const uint32_t s) {
         const int8_t *as = a_base + (size_t) s * STAGE_K, *bs = b_base + (size_t) s * STAGE_K;
 #pragma unroll
-        for (int i = 0; i < NLA; ++i) ra[i] = load16<ALIGNED>(as + a_at[i]);
+        for (int i = 0; i < NLA; ++i) ra[i] = load16(as + a_at[i]);
 #pragma unroll
-        for (int i = 0; i < NLB; ++i) rb[i] = load16<ALIGNED>(bs + b_at[i]);
+        for (int i = 0; i < NLB; ++i) rb[i] = load16(bs + b_at[i]);
     };
     const auto request_last = [&](const uint32_t s) {  // a stage that the rows end in
         const int k = (int) (s * STAGE_K + ld_chunk * 16);
@@ -437,17 +487,16 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
 }
 
 template <class O, int RT, int NB, int WAVES, int AHEAD>
-int launch_few_rows(skm_ctx* ctx, const ProductArgs& p, const bool aligned) {
+int launch_few_rows(skm_ctx* ctx, const ProductArgs& p) {
     const uint32_t tiles_n = (p.n + 16 * NB - 1) / (16 * NB);
     const uint64_t blocks = ((uint64_t) (p.m + 16 * RT - 1) / (16 * RT) + (p.offsets ? p.groups : 0)) * tiles_n;
     if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
-    if (aligned) product_few_rows_kernel<O, RT, NB, WAVES, AHEAD, true><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
-    else product_few_rows_kernel<O, RT, NB, WAVES, AHEAD, false><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
+    product_few_rows_kernel<O, RT, NB, WAVES, AHEAD><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
     return check_hip(hipGetLastError(), "product_few_rows_kernel launch");
 }
 
 template <class O, int FM, int FN>
-int launch_tiles(skm_ctx* ctx, const ProductArgs& p, const bool aligned) {
+int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
     constexpr size_t lds = tiles_lds_bytes<FM, FN>();
     const uint32_t tiles_n = (p.n + 64 * FN - 1) / (64 * FN);
     const uint64_t tiles_m = (uint64_t) (p.m + 64 * FM - 1) / (64 * FM) + (p.offsets ? p.groups : 0);
@@ -463,7 +512,7 @@ int launch_tiles(skm_ctx* ctx, const ProductArgs& p, const bool aligned) {
         kernel<<<(unsigned) blocks, 256, lds, ctx->stream>>>(p, map);
         return check_hip(hipGetLastError(), "product_tiles_kernel launch");
     };
-    return aligned ? launch(product_tiles_kernel<O, FM, FN, true>) : launch(product_tiles_kernel<O, FM, FN, false>);
+    return launch(product_tiles_kernel<O, FM, FN>);
 }
 
 } // namespace
@@ -493,10 +542,17 @@ int skm_quantize_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t 
         using T = decltype(sample);
         return for_width<T>(per_lane * size, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const unsigned blocks = (unsigned) std::min<uint64_t>(n, ROWS_MAX_BLOCKS);
-            quantize_rows_kernel<T, E><<<blocks, QUANTIZE_THREADS, 0, ctx->stream>>>((const T*) d_x, n, (uint32_t) (d / E), x_stride, d_q,
-                                                                                     q_stride, d_scales);
-            return check_hip(hipGetLastError(), "quantize_rows_kernel launch");
+            const uint32_t vectors = (uint32_t) (d / E);
+            const auto launch = [&](auto waves, auto held) {
+                constexpr int WAVES = decltype(waves)::value, HELD = decltype(held)::value, ROWS = QUANTIZE_THREADS / 64 / WAVES;
+                const unsigned blocks = (unsigned) std::min<uint64_t>((n + ROWS - 1) / ROWS, ROWS_MAX_BLOCKS);
+                quantize_rows_kernel<T, E, WAVES, HELD><<<blocks, QUANTIZE_THREADS, 0, ctx->stream>>>((const T*) d_x, n, vectors, x_stride,
+                                                                                                      d_q, q_stride, d_scales);
+                return check_hip(hipGetLastError(), "quantize_rows_kernel launch");
+            };
+            if (vectors <= 256) return launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+            if (vectors <= 512) return launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+            return launch(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
         });
     });
 }
@@ -526,18 +582,17 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
     ScopedStage st(ctx, "rows/product");
     const ProductArgs p{d_a, d_a_scale, d_b, d_b_scale, d_bias, d_offsets, d_out, a_stride, b_stride, d_offsets ? b_group_stride : 0,
                         out_stride, (uint32_t) m, (uint32_t) n, (uint32_t) k, d_offsets ? (uint32_t) groups : 1};
-    const bool aligned = common_width({address(d_a), address(d_b), a_stride, b_stride, p.b_group_stride}) == 16;
     return for_type(out_type, [&](auto sample) {
         using O = decltype(sample);
         const size_t rows = d_offsets ? (m + groups - 1) / groups : m;  // of a group, on average
         const bool near = k >= 16 && a_stride < (1u << 23) && b_stride < (1u << 23);  // as the tiles' loads assume (32-bit offsets)
         const uint64_t parts = d_offsets ? groups : 1;
         const uint64_t large = parts * ((rows + 255) / 256) * ((n + 255) / 256), medium = parts * ((rows + 127) / 128) * ((n + 127) / 128);
-        if (near && rows > 128 && large >= 192) return launch_tiles<O, 4, 4>(ctx, p, aligned);
-        if (near && rows > 64 && medium >= 128) return launch_tiles<O, 2, 2>(ctx, p, aligned);
-        if (rows > 16) return launch_few_rows<O, 4, 2, 8, 2>(ctx, p, aligned);
-        if (rows > 4) return launch_few_rows<O, 2, 2, 8, 4>(ctx, p, aligned);
-        return launch_few_rows<O, 1, 2, 8, 4>(ctx, p, aligned);
+        if (near && rows > 128 && large >= 192) return launch_tiles<O, 4, 4>(ctx, p);
+        if (near && rows > 64 && medium >= 128) return launch_tiles<O, 2, 2>(ctx, p);
+        if (rows > 16) return launch_few_rows<O, 4, 2, 8, 2>(ctx, p);
+        if (rows > 4) return launch_few_rows<O, 2, 2, 4, 4>(ctx, p);
+        return launch_few_rows<O, 1, 1, 8, 8>(ctx, p);
     });
 }
 
