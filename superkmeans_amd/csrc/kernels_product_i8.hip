@@ -62,7 +62,7 @@ constexpr int QUANTIZE_THREADS = 256;
 
 template <class T, int E, int WAVES, int HELD>
 __global__ __launch_bounds__(QUANTIZE_THREADS) void quantize_rows_kernel(
-    const T* __restrict__ x, const size_t n, const uint32_t vectors, const size_t x_stride, int8_t* __restrict__ q,
+    const T* __restrict__ x, const size_t n, const uint32_t vectors, const uint32_t last, const size_t x_stride, int8_t* __restrict__ q,
     const size_t q_stride, float* __restrict__ scales
 ) {
     constexpr int ROWS = QUANTIZE_THREADS / 64 / WAVES, LANES = 64 * WAVES;  // ROWS per workgroup
@@ -80,11 +80,11 @@ __global__ __launch_bounds__(QUANTIZE_THREADS) void quantize_rows_kernel(
         vec_of<T, E> held[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (in_row + i * LANES < mine) held[i] = load_vec<T, E>(row + (size_t) (in_row + i * LANES) * E);
+            if (in_row + i * LANES < mine) held[i] = load_vec<T, E>(row + column<E>(in_row + i * LANES, last));
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
             if (in_row + i * LANES < mine) look(held[i]);
-        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) look(load_vec<T, E>(row + (size_t) at * E));
+        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) look(load_vec<T, E>(row + column<E>(at, last)));
         auto one = largest[0];
 #pragma unroll
         for (int e = 1; e < E; ++e) one = one > largest[e] ? one : largest[e];
@@ -104,12 +104,12 @@ __global__ __launch_bounds__(QUANTIZE_THREADS) void quantize_rows_kernel(
         if (in_row == 0 && t < n) scales[t] = most < 0x7f800000u ? m / 127.0f : __builtin_nanf("");
         const auto put = [&](const uint32_t at, const vec_of<T, E> v) {
             const vec_of<int8_t, E> r = usable ? nearest_steps<E>(widen<E>(v), m, inverse) : vec_of<int8_t, E>{};
-            *reinterpret_cast<vec_of<int8_t, E>*>(q + t * q_stride + (size_t) at * E) = r;
+            store_vec<int8_t, E>(q + t * q_stride + column<E>(at, last), r);
         };
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
             if (in_row + i * LANES < mine) put(in_row + i * LANES, held[i]);
-        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) put(at, load_vec<T, E>(row + (size_t) at * E));
+        for (uint32_t at = in_row + HELD * LANES; at < mine; at += LANES) put(at, load_vec<T, E>(row + column<E>(at, last)));
     }
 }
 
@@ -536,17 +536,15 @@ int skm_quantize_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t 
     SKM_REQUIRE(!overlap(d_x, span(n, x_stride, d, size), d_q, span(n, q_stride, d, 1)), "q overlaps x");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/quantize");
-    const size_t in_width = common_width({address(d_x), x_stride * size, d * size});
-    const size_t per_lane = std::min(in_width / size, common_width({address(d_q), q_stride, d}));
     return for_type(type, [&](auto sample) {
         using T = decltype(sample);
-        return for_width<T>(per_lane * size, [&](auto elements) {
+        return for_elements<T>(vector_elements(size, 1, d), [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const uint32_t vectors = (uint32_t) (d / E);
+            const uint32_t vectors = (uint32_t) ((d + E - 1) / E);
             const auto launch = [&](auto waves, auto held) {
                 constexpr int WAVES = decltype(waves)::value, HELD = decltype(held)::value, ROWS = QUANTIZE_THREADS / 64 / WAVES;
                 const unsigned blocks = (unsigned) std::min<uint64_t>((n + ROWS - 1) / ROWS, ROWS_MAX_BLOCKS);
-                quantize_rows_kernel<T, E, WAVES, HELD><<<blocks, QUANTIZE_THREADS, 0, ctx->stream>>>((const T*) d_x, n, vectors, x_stride,
+                quantize_rows_kernel<T, E, WAVES, HELD><<<blocks, QUANTIZE_THREADS, 0, ctx->stream>>>((const T*) d_x, n, vectors, (uint32_t) (d - E), x_stride,
                                                                                                       d_q, q_stride, d_scales);
                 return check_hip(hipGetLastError(), "quantize_rows_kernel launch");
             };

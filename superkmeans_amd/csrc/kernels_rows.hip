@@ -58,7 +58,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i) {
                 const uint32_t at = first + i * s.lanes;
-                if (at < s.vectors && id[q] < rows) v[q][i] = load_vec<T, E>(table + id[q] * table_stride + (size_t) at * E);
+                if (at < s.vectors && id[q] < rows) v[q][i] = load_vec<T, E>(table + id[q] * table_stride + column<E>(at, s.last));
                 else v[q][i] = vec_of<T, E>{};
             }
 #pragma unroll
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
                 const uint32_t at = first + i * s.lanes;
                 if (at < s.vectors) {
                     const vec_of<T, E> r = scale == 1.0f || id[q] >= rows ? v[q][i] : narrow<T, E>(widen<E>(v[q][i]) * scale);
-                    store_vec_once<T, E>(out + (t + q * rows_of_wave) * out_stride + (size_t) at * E, r);
+                    store_vec_once<T, E>(out + (t + q * rows_of_wave) * out_stride + column<E>(at, s.last), r);
                 }
             }
         }
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) {
             const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors) v[i] = load_vec_once<T, E>(x + t * x_stride + (size_t) at * E);
+            if (at < s.vectors) v[i] = load_vec_once<T, E>(x + t * x_stride + column<E>(at, s.last));
         }
         for (uint32_t j = 0; j < choices; ++j) {
             const uint32_t slot = slots[t * choices + j];
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
 #pragma unroll
             for (int i = 0; i < UNROLL; ++i) {
                 const uint32_t at = first + i * s.lanes;
-                if (at < s.vectors) store_vec_once<T, E>(out + (size_t) slot * out_stride + (size_t) at * E, v[i]);
+                if (at < s.vectors) store_vec_once<T, E>(out + (size_t) slot * out_stride + column<E>(at, s.last), v[i]);
             }
         }
     }
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
                 for (int i = 0; i < COMBINE_UNROLL; ++i) {
                     const uint32_t at = first + i * s.lanes;
                     if (slot[j] < n_rows && at < s.vectors)
-                        v[j][i] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                        v[j][i] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + column<E>(at, s.last));
                 }
 #pragma unroll
             for (int j = 0; j < COMBINE_AHEAD; ++j)
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
 #pragma unroll
         for (int i = 0; i < COMBINE_UNROLL; ++i) {
             const uint32_t at = first + i * s.lanes;
-            if (at < s.vectors) store_vec_once<T, E>(out + t * out_stride + (size_t) at * E, narrow<T, E>(sum[i]));
+            if (at < s.vectors) store_vec_once<T, E>(out + t * out_stride + column<E>(at, s.last), narrow<T, E>(sum[i]));
         }
     }
 }
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
 // for each GRAD_CHOICES choices, WAVES wavefronts per token.
 template <class T, int E, int WAVES, int GRAD_CHOICES>
 __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
-    const T* __restrict__ grad, const size_t n, const uint32_t vectors, const size_t grad_stride, const T* __restrict__ rows,
+    const T* __restrict__ grad, const size_t n, const uint32_t vectors, const uint32_t last, const size_t grad_stride, const T* __restrict__ rows,
     const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const uint32_t choices,
     const void* __restrict__ weights, const int weights_type, T* __restrict__ grad_rows, const size_t grad_rows_stride,
     void* __restrict__ grad_weights
@@ -195,12 +195,14 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
                     if (weights && slot[j] < n_rows) w[j] = weight_at(weights, weights_type, t * choices + j0 + j);
                 }
                 for (uint32_t at = in_row; at < vectors; at += 64 * WAVES) {
-                    const vec_of<float, E> g = widen<E>(load_vec<T, E>(grad + t * grad_stride + (size_t) at * E));
+                    const uint32_t c = column<E>(at, last);
+                    const int repeated = (int) (at * E - c);  // elements that the vector before has too
+                    const vec_of<float, E> g = widen<E>(load_vec<T, E>(grad + t * grad_stride + c));
                     vec_of<T, E> y[GRAD_CHOICES];
                     if (grad_weights) {
 #pragma unroll
                         for (int j = 0; j < GRAD_CHOICES; ++j)
-                            if (slot[j] < n_rows) y[j] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + (size_t) at * E);
+                            if (slot[j] < n_rows) y[j] = load_vec_once<T, E>(rows + (size_t) slot[j] * rows_stride + c);
                     }
 #pragma unroll
                     for (int j = 0; j < GRAD_CHOICES; ++j) {
@@ -209,11 +211,11 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
                             const vec_of<float, E> p = g * widen<E>(y[j]);
                             float sum = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < E; ++e) sum += p[e];
+                            for (int e = 0; e < E; ++e) sum += e >= repeated ? p[e] : 0.0f;
                             dot[j] += sum;
                         }
                         if (grad_rows)
-                            store_vec_once<T, E>(grad_rows + (size_t) slot[j] * grad_rows_stride + (size_t) at * E, narrow<T, E>(g * w[j]));
+                            store_vec_once<T, E>(grad_rows + (size_t) slot[j] * grad_rows_stride + c, narrow<T, E>(g * w[j]));
                     }
                 }
             }
@@ -267,20 +269,19 @@ int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, si
     SKM_REQUIRE(!overlap(d_table, span(rows, table_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the table");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup");
-    const size_t width = common_width({address(d_table), address(d_out), table_stride * size, out_stride * size, d * size});
     return for_type(type, [&](auto sample) {
         using T = decltype(sample);
-        return for_width<T>(width, [&](auto elements) {
+        return for_elements<T>(vector_elements(size, size, d), [&](auto elements) {
             constexpr int E = decltype(elements)::value;
             const auto launch = [&](auto tokens) {
                 constexpr int TOKENS = decltype(tokens)::value;
-                const RowSplit s = split_rows((n + TOKENS - 1) / TOKENS, d / E, UNROLL);
+                const RowSplit s = split_rows((n + TOKENS - 1) / TOKENS, d, E, UNROLL);
                 lookup_rows_kernel<T, E, TOKENS><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
                     (const T*) d_table, rows, table_stride, d_ids, ids_type, n, scale, (T*) d_out, out_stride, s);
                 return check_hip(hipGetLastError(), "lookup_rows_kernel launch");
             };
             // several rows to a wavefront once there are wavefronts for the whole chip all the same (32 on each compute unit)
-            if (split_rows(n, d / E, UNROLL).units >= 4 * 8192) return launch(std::integral_constant<int, 4>{});
+            if (split_rows(n, d, E, UNROLL).units >= 4 * 8192) return launch(std::integral_constant<int, 4>{});
             return launch(std::integral_constant<int, 1>{});
         });
     });
@@ -302,12 +303,11 @@ int skm_dispatch_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t 
     SKM_REQUIRE(!overlap(d_x, span(n, x_stride, d, size), d_out, span(out_rows, out_stride, d, size)), "out overlaps x");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/dispatch");
-    const size_t width = common_width({address(d_x), address(d_out), x_stride * size, out_stride * size, d * size});
     return for_type(type, [&](auto sample) {
         using T = decltype(sample);
-        return for_width<T>(width, [&](auto elements) {
+        return for_elements<T>(vector_elements(size, size, d), [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const RowSplit s = split_rows(n, d / E, UNROLL);
+            const RowSplit s = split_rows(n, d, E, UNROLL);
             dispatch_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
                 (const T*) d_x, x_stride, n, d_slots, (uint32_t) choices, out_rows, (T*) d_out, out_stride, s);
             return check_hip(hipGetLastError(), "dispatch_rows_kernel launch");
@@ -333,12 +333,11 @@ int skm_combine_rows(skm_ctx* ctx, const void* d_rows, int type, size_t n_rows, 
     SKM_REQUIRE(!overlap(d_rows, span(n_rows, rows_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the rows");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/combine");
-    const size_t width = common_width({address(d_rows), address(d_out), rows_stride * size, out_stride * size, d * size});
     return for_type(type, [&](auto sample) {
         using T = decltype(sample);
-        return for_width<T>(width, [&](auto elements) {
+        return for_elements<T>(vector_elements(size, size, d), [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const RowSplit s = split_rows(n, d / E, COMBINE_UNROLL);
+            const RowSplit s = split_rows(n, d, E, COMBINE_UNROLL);
             combine_rows_kernel<T, E><<<row_blocks(s), ROWS_THREADS, 0, ctx->stream>>>(
                 (const T*) d_rows, n_rows, rows_stride, d_slots, n, (uint32_t) choices, d_weights, weights_type, (T*) d_out,
                 out_stride, s);
@@ -372,20 +371,17 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
     }
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/combine_grad");
-    size_t width = common_width({address(d_grad), grad_stride * size, d * size});
-    if (d_grad_weights) width = std::min(width, common_width({address(d_rows), rows_stride * size}));
-    if (d_grad_rows) width = std::min(width, common_width({address(d_grad_rows), grad_rows_stride * size}));
     return for_type(type, [&](auto sample) {
         using T = decltype(sample);
-        return for_width<T>(width, [&](auto elements) {
+        return for_elements<T>(vector_elements(size, size, d), [&](auto elements) {
             constexpr int E = decltype(elements)::value;
-            const uint32_t vectors = (uint32_t) (d / E);
+            const uint32_t vectors = (uint32_t) ((d + E - 1) / E);
             const auto launch = [&](auto waves, auto together) {
                 constexpr int WAVES = decltype(waves)::value;
                 const size_t turns = (n + ROWS_THREADS / 64 / WAVES - 1) / (ROWS_THREADS / 64 / WAVES);
                 const unsigned blocks = (unsigned) std::min<uint64_t>(ROWS_MAX_BLOCKS, turns);
                 combine_rows_grad_kernel<T, E, WAVES, decltype(together)::value><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
-                    (const T*) d_grad, n, vectors, grad_stride, (const T*) d_rows, n_rows, rows_stride, d_slots, (uint32_t) choices,
+                    (const T*) d_grad, n, vectors, (uint32_t) (d - E), grad_stride, (const T*) d_rows, n_rows, rows_stride, d_slots, (uint32_t) choices,
                     d_weights, weights_type, (T*) d_grad_rows, grad_rows_stride, d_grad_weights);
                 return check_hip(hipGetLastError(), "combine_rows_grad_kernel launch");
             };

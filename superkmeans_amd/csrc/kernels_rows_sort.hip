@@ -348,7 +348,7 @@ struct GradArgs {
     size_t out_stride;
     float scale;
     bool accumulate;
-    uint32_t n, rows, vectors, pieces;  // vectors per row; pieces of 64 vectors
+    uint32_t n, rows, d, vectors, last, pieces;  // vectors per row, the last one's column; pieces of 64 vectors
     // sorted tokens: their keys and positions, in chunks of `chunk`, and the chunks' sums of rows that go past them
     const uint32_t *keys, *index;
     uint32_t chunk, chunks;
@@ -380,8 +380,8 @@ __device__ __forceinline__ void grad_of_chunk(const GradArgs& g, const RowSplit&
         for (int i = 0; i < GRAD_VECTORS; ++i) {
             const uint32_t at = first + i * s.lanes;
             if (at < g.vectors) {
-                if (whole && ends) put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) row * g.out_stride + (size_t) at * E, sum[i], g.scale, g.accumulate);
-                else store_vec<float, E>(g.parts + ((size_t) c * 2 + slot) * g.vectors * E + (size_t) at * E, sum[i]);
+                if (whole && ends) put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) row * g.out_stride + column<E>(at, g.last), sum[i], g.scale, g.accumulate);
+                else store_vec<float, E>(g.parts + ((size_t) c * 2 + slot) * g.d + column<E>(at, g.last), sum[i]);
             }
             sum[i] = vec_of<float, E>{};
         }
@@ -401,7 +401,7 @@ __device__ __forceinline__ void grad_of_chunk(const GradArgs& g, const RowSplit&
 #pragma unroll
             for (int i = 0; i < GRAD_VECTORS; ++i) {
                 const uint32_t at = first + i * s.lanes;
-                if (at < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) token[q] * g.grad_stride + (size_t) at * E);
+                if (at < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) token[q] * g.grad_stride + column<E>(at, g.last));
             }
 #pragma unroll
         for (int q = 0; q < GRAD_AHEAD; ++q) {
@@ -438,7 +438,7 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit
     }
     for (unsigned long long left = __ballot(empty); left; left &= left - 1) {
         O* out = reinterpret_cast<O*>(g.out) + (size_t) (unit * FILL_ROWS + (uint32_t) __builtin_ctzll(left)) * g.out_stride;
-        for (uint32_t at = lane; at < g.vectors; at += 64) store_vec_once<O, E>(out + (size_t) at * E, vec_of<O, E>{});
+        for (uint32_t at = lane; at < g.vectors; at += 64) store_vec_once<O, E>(out + column<E>(at, g.last), vec_of<O, E>{});
     }
 }
 
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(const Gr
     constexpr int WAVES = ROWS_THREADS / 64;
     __shared__ vec_of<float, E> share[WAVES][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const size_t stride = (size_t) 2 * g.vectors * E;
+    const size_t stride = (size_t) 2 * g.d;
     uint32_t c, piece;
     Crossing x;
     const bool alone = blockIdx.x < alone_blocks;
@@ -519,7 +519,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(const Gr
     const uint32_t p0 = alone ? 0 : min(wave * each, x.parts), p1 = min(p0 + each, x.parts);
     vec_of<float, E> sum = {};
     if (at < g.vectors) {
-        const float* part = g.parts + c * stride + (size_t) at * E;
+        const float* part = g.parts + c * stride + column<E>(at, g.last);
 #pragma unroll 8
         for (uint32_t p = p0; p < p1; ++p) sum += load_vec<float, E>(part + p * stride + (p == 0 && !x.at_start ? stride / 2 : 0));
     }
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(const Gr
         for (int w = 1; w < WAVES && wave == 0; ++w) sum += share[w][lane];
     }
     if ((alone || wave == 0) && at < g.vectors)
-        put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + (size_t) at * E, sum, g.scale, g.accumulate);
+        put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + column<E>(at, g.last), sum, g.scale, g.accumulate);
 }
 
 // Few tokens: one launch and no sort.  A workgroup owns every `step`-th row, reads all ids, and lists the tokens of its rows in order
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
                         same &= same - 1;
 #pragma unroll
                         for (int i = 0; i < V; ++i)
-                            if (at + i * 64 < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) t * g.grad_stride + (size_t) (at + i * 64) * E);
+                            if (at + i * 64 < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) t * g.grad_stride + column<E>(at + i * 64, g.last));
                         taken = q + 1;
                     }
                 }
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
         O* out = reinterpret_cast<O*>(g.out) + (size_t) (r * step + blockIdx.x) * g.out_stride;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (at + i * 64 < g.vectors) put_sum<O, E>(out + (size_t) (at + i * 64) * E, sum[i], g.scale, g.accumulate);
+            if (at + i * 64 < g.vectors) put_sum<O, E>(out + column<E>(at + i * 64, g.last), sum[i], g.scale, g.accumulate);
     };
     const uint32_t pieces = (g.vectors + 64 * V - 1) / (64 * V);
     for (uint32_t u = wave; u < mine * pieces; u += WAVES) {
@@ -720,15 +720,13 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
     SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_out, span(rows, out_stride, d, out_size)), "out overlaps the gradient");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup_grad");
-    // elements per lane: what the alignment of both sides gives in one load and one store of at most 16 bytes
-    const size_t in_width = common_width({address(d_grad), grad_stride * size, d * size});
-    const size_t out_width = common_width({address(d_out), out_stride * out_size, d * out_size});
-    const size_t per_lane = std::min(in_width / size, out_width / out_size);
+    // an accumulated vector must not be added twice
+    const size_t per_lane = vector_elements(size, out_size, d, accumulate != 0);
     const KeySource source{d_ids, ids_type, (uint32_t) rows};
     const auto run = [&](auto sample, auto out_sample) {
         using T = decltype(sample);
         using O = decltype(out_sample);
-        return for_width<T>(per_lane * size, [&](auto elements) {
+        return for_elements<T>(per_lane, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
             GradArgs g{};
             g.grad = d_grad;
@@ -739,7 +737,9 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
             g.accumulate = accumulate != 0;
             g.n = (uint32_t) n;
             g.rows = (uint32_t) rows;
-            g.vectors = (uint32_t) (d / E);
+            g.d = (uint32_t) d;
+            g.vectors = (uint32_t) ((d + E - 1) / E);
+            g.last = (uint32_t) (d - E);
             g.pieces = (g.vectors + 63) / 64;
             if (n <= FEW_TOKENS) {
                 // a workgroup per row up to 1,024, then a few rows each: reading the ids costs a workgroup about as much as two rows
@@ -757,7 +757,7 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
             g.chunk = plan.chunk;
             g.chunks = plan.chunks;
             g.parts = (float*) (scratch + plan.at_parts);
-            const RowSplit s = split_rows(plan.chunks, g.vectors, GRAD_VECTORS);
+            const RowSplit s = split_rows(plan.chunks, d, E, GRAD_VECTORS);
             constexpr uint64_t PER_BLOCK = ROWS_THREADS / 64;
             const uint64_t chunk_blocks = (s.units + PER_BLOCK - 1) / PER_BLOCK;
             const uint64_t fill_units = accumulate ? 0 : (rows + FILL_ROWS - 1) / FILL_ROWS;
