@@ -313,12 +313,16 @@ constexpr size_t tiles_lds_bytes() {
 }
 
 // Number of a workgroup to tile: workgroups whose number is equal mod 8 run on the same die and share its L2, where 32 of them
-// at a time take a block of `super_m` x 32 / super_m neighbouring tiles.
+// at a time take a block of `super_m` x 32 / super_m neighbouring tiles.  The blocks that do not go round the eight dies (from
+// number `even` on) are dealt out tile by tile, so that no die has a block more than another.
 struct TileMap {
-    uint32_t super_m, super_n, across, tiles_n;
+    uint32_t super_m, super_n, across, tiles_n, even;
     __device__ __forceinline__ bool operator()(const uint32_t number, uint32_t& tile_m, uint32_t& tile_n) const {
-        const uint32_t die = number & 7, local = number >> 3;
-        const uint32_t super = (local >> 5) * 8 + die, within = local & 31;
+        uint32_t super = number >> 5, within = number & 31;
+        if (number < even) {
+            super = (number >> 8) * 8 + (number & 7);
+            within = (number >> 3) & 31;
+        }
         tile_m = super / across * super_m + within % super_m;
         tile_n = super % across * super_n + within / super_m;
         return tile_n < tiles_n;
@@ -397,11 +401,11 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     // slice's products, when every read of the stage has returned, and the next stage's first slice is read under them.
     // (Left to itself the compiler reads a slice right before its products: 3 % more time.)
     const auto interleave = [] {
-        if constexpr (FM == 4 && FN == 4) {
+        if constexpr (FM * FN >= 2 * (FM + FN)) {
 #pragma unroll
             for (int i = 0; i < FM + FN; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);  // matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x008, FM * FN / (FM + FN), 0);  // matrix instructions
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -451,7 +455,6 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     }
     __syncthreads();
     O* out = reinterpret_cast<O*>(p.out);
-    const bool wide = ((reinterpret_cast<size_t>(out) | p.out_stride * sizeof(O)) & 15) == 0;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const uint32_t m0 = rows.first + wm + i * 32;
@@ -476,7 +479,7 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
             if (m >= rows.end || n >= p.n) continue;
             const vec_of<O, E> v = *reinterpret_cast<const vec_of<O, E>*>(&staged[r * LD + c]);
             O* to = out + (size_t) m * p.out_stride + n;
-            if (wide && n + E <= p.n) *reinterpret_cast<vec_of<O, E>*>(to) = v;
+            if (n + E <= p.n) store_vec_once<O, E>(to, v);
             else
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -503,9 +506,9 @@ int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
     uint32_t super_n = 1;
     while (super_n < 8 && super_n < tiles_n) super_n *= 2;
     const uint32_t super_m = 32 / super_n, across = (tiles_n + super_n - 1) / super_n;
-    const uint64_t supers = (tiles_m + super_m - 1) / super_m * across, blocks = (supers + 7) / 8 * 8 * 32;
+    const uint64_t supers = (tiles_m + super_m - 1) / super_m * across, blocks = supers * 32;
     if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
-    const TileMap map{super_m, super_n, across, tiles_n};
+    const TileMap map{super_m, super_n, across, tiles_n, (uint32_t) (supers / 8 * 256)};
     const auto launch = [&](auto kernel) {
         SKM_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds),
                           "hipFuncSetAttribute(MaxDynamicSharedMemorySize)"));
@@ -513,6 +516,46 @@ int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
         return check_hip(hipGetLastError(), "product_tiles_kernel launch");
     };
     return launch(product_tiles_kernel<O, FM, FN>);
+}
+
+// The kernel for a call: the largest tile that still gives every compute unit a workgroup.  A larger tile reads each operand
+// fewer times, and loses more than that where it leaves compute units without one (us, bf16 results):
+//     rows x n x k          256 x 256  128 x 128  128 x 64  64 x 64    few rows: 32 x 64  32 x 32  32 x 16  16 x 16
+//     8192 x 8192 x 4096       287        333        412      507
+//     1024 x 4096 x 4096        72         30         34       37
+//      512 x 4096 x 4096                   27         19       20                   50
+//      256 x 4096 x 4096                   24         18       15                   26
+//      128 x 4096 x 4096                              18       15                   14       17
+//       64 x 4096 x 4096                                       15                   14       10       12       12
+//       64 x 1024 x 4096                                                                     10        8        7
+//        1 x 4096 x 4096                                                                      8        7        7
+// Over groups the host knows the rows of a group on average only.  There 64 x 64 tiles pay from 9 rows on (64 groups, n 2048,
+// k 1024: 16 rows each 27 us against 36 us with few rows' kernel, 8 rows each 27 with 16 x 64 of it and more with tiles), and the
+// 256 x 256 tiles never, as the groups' ends leave half a tile each (8 groups, 32768 x 4096 x 1536: 294 against 307 us).
+template <class O>
+int launch_product(skm_ctx* ctx, const ProductArgs& p) {
+    constexpr uint64_t WANTED = 256;
+    const bool grouped = p.offsets != nullptr;
+    const uint64_t rows = ((uint64_t) p.m + p.groups - 1) / p.groups;  // of a group, on average
+    const auto tiles = [&](const uint64_t tm, const uint64_t tn) { return p.groups * ((rows + tm - 1) / tm) * ((p.n + tn - 1) / tn); };
+    // what the tiles' loads assume: 16 columns at least, a tile's offsets in 32 bits
+    if (p.k >= 16 && p.a_stride < (1u << 23) && p.b_stride < (1u << 23)) {
+        // The large tiles run one to a compute unit, so a last round that is partly filled takes as long as a full one; the medium
+        // ones run two to a unit and drift apart.  Microseconds of a round by the columns, from products of whole rounds.
+        const double columns = p.k / 1024.0;
+        const double large = (double) ((tiles(256, 256) + 255) / 256) * (10.0 + 15.0 * columns);
+        const double medium = std::max(1.0, tiles(128, 128) / 512.0 + 0.25) * (4.0 + 9.4 * columns);
+        if (!grouped && tiles(256, 256) >= WANTED && large <= medium) return launch_tiles<O, 4, 4>(ctx, p);
+        if (rows > 64 && tiles(128, 128) >= WANTED) return launch_tiles<O, 2, 2>(ctx, p);
+        if (rows > 64 && tiles(128, 64) >= WANTED) return launch_tiles<O, 2, 1>(ctx, p);
+        if (rows > (grouped ? 8 : 32) && tiles(64, 64) >= WANTED) return launch_tiles<O, 1, 1>(ctx, p);
+    }
+    if (rows > 16 && tiles(32, 64) >= WANTED) return launch_few_rows<O, 2, 4, 8, 2>(ctx, p);
+    if (rows > 16 && tiles(32, 32) >= WANTED) return launch_few_rows<O, 2, 2, 8, 4>(ctx, p);
+    if (rows > 16) return launch_few_rows<O, 2, 1, 8, 4>(ctx, p);
+    if (grouped && tiles(16, 64) >= 4 * WANTED) return launch_few_rows<O, 1, 4, 4, 4>(ctx, p);
+    if (grouped) return launch_few_rows<O, 2, 2, 4, 4>(ctx, p);
+    return launch_few_rows<O, 1, 1, 8, 8>(ctx, p);
 }
 
 } // namespace
@@ -582,15 +625,7 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
                         out_stride, (uint32_t) m, (uint32_t) n, (uint32_t) k, d_offsets ? (uint32_t) groups : 1};
     return for_type(out_type, [&](auto sample) {
         using O = decltype(sample);
-        const size_t rows = d_offsets ? (m + groups - 1) / groups : m;  // of a group, on average
-        const bool near = k >= 16 && a_stride < (1u << 23) && b_stride < (1u << 23);  // as the tiles' loads assume (32-bit offsets)
-        const uint64_t parts = d_offsets ? groups : 1;
-        const uint64_t large = parts * ((rows + 255) / 256) * ((n + 255) / 256), medium = parts * ((rows + 127) / 128) * ((n + 127) / 128);
-        if (near && rows > 128 && large >= 192) return launch_tiles<O, 4, 4>(ctx, p);
-        if (near && rows > 64 && medium >= 128) return launch_tiles<O, 2, 2>(ctx, p);
-        if (rows > 16) return launch_few_rows<O, 4, 2, 8, 2>(ctx, p);
-        if (rows > 4) return launch_few_rows<O, 2, 2, 4, 4>(ctx, p);
-        return launch_few_rows<O, 1, 1, 8, 8>(ctx, p);
+        return launch_product<O>(ctx, p);
     });
 }
 
