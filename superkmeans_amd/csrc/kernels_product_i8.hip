@@ -134,38 +134,31 @@ struct RowTile {
     uint32_t group, first, end;
 };
 
-// The tile of `tm` rows with the given number, counted through the groups; first == end where there is none.  Offsets are
-// clamped to the rows there are.  Every wavefront of a workgroup finds it by itself, 64 groups at a time.
-__device__ __forceinline__ RowTile find_rows(const ProductArgs& p, const uint32_t tm, uint32_t number) {
+// The tile of `tm` rows with the given number; first >= end where there is none.  Group g has the numbers from
+// offsets[g] / tm + g on: as many as its rows can need, whatever the other groups hold, so that the group of a number is found by
+// a search and the numbers of all groups end at m / tm + groups.  Every wavefront of a workgroup looks by itself, at 64 groups
+// at a time.  Offsets are clamped to the rows there are.
+__device__ __forceinline__ RowTile find_rows(const ProductArgs& p, const uint32_t tm, const uint32_t number) {
     if (!p.offsets) {
         const uint32_t first = number * tm;
         return {0, min(first, p.m), min(p.m, first + tm)};
     }
     const uint32_t lane = threadIdx.x & 63;
-    for (uint32_t g0 = 0; g0 < p.groups; g0 += 64) {
-        const uint32_t g = g0 + lane;
-        uint32_t from = 0, to = 0;
-        if (g < p.groups) {
-            from = min(p.offsets[g], p.m);
-            to = max(from, min(p.offsets[g + 1], p.m));
-        }
-        const uint32_t tiles = (to - from + tm - 1) / tm;
-        uint32_t incl = tiles;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t t = __shfl_up(incl, off);
-            if (lane >= (uint32_t) off) incl += t;
-        }
-        const unsigned long long past = __ballot(incl > number);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            const uint32_t before = __shfl(incl - tiles, at);
-            const uint32_t first = __shfl(from, at) + (number - before) * tm;
-            return {g0 + at, first, min((uint32_t) __shfl(to, at), first + tm)};
-        }
-        number -= __shfl(incl, 63);
+    uint32_t low = 0, many = p.groups;  // the group is one of `many` from `low` on
+    for (;;) {
+        const uint32_t step = (many + 63) / 64, g = low + lane * step;
+        const bool begun = lane * step < many && min(p.offsets[g], p.m) / tm + g <= number;
+        const unsigned long long before = __ballot(begun);
+        if (!before) return {0, 0, 0};
+        const uint32_t at = 63 - (uint32_t) __builtin_clzll(before);
+        low += at * step;
+        many = min(step, many - at * step);
+        if (step == 1) break;
     }
-    return {0, 0, 0};
+    const uint32_t from = min(p.offsets[low], p.m), to = min(p.offsets[low + 1], p.m);
+    const uint64_t first = (uint64_t) from + (uint64_t) (number - from / tm - low) * tm;
+    if (first >= to) return {0, 0, 0};
+    return {low, (uint32_t) first, (uint32_t) min((uint64_t) to, first + tm)};
 }
 
 // 16 bytes of a row, at any address: the load instruction takes them unaligned too, only the compiler has to be told.
@@ -618,6 +611,8 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
                 "pointers must be aligned to their elements");
     const size_t out_bytes = span(m, out_stride, n, out_size);
     SKM_REQUIRE(!overlap(d_a, span(m, a_stride, k, 1), d_out, out_bytes), "out overlaps a");
+    SKM_REQUIRE(!overlap(d_a_scale, m * 4, d_out, out_bytes) && !overlap(d_b_scale, (d_offsets ? groups : 1) * n * 4, d_out, out_bytes),
+                "out overlaps the scales");
     SKM_REQUIRE(!overlap(d_b, (d_offsets ? (groups - 1) * b_group_stride : 0) + span(n, b_stride, k, 1), d_out, out_bytes), "out overlaps b");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/product");

@@ -266,7 +266,8 @@ int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, si
     const size_t size = type_size(type);
     SKM_REQUIRE(address(d_ids) % (ids_type == SKM_I64 ? 8 : 4) == 0 && address(d_table) % size == 0 && address(d_out) % size == 0,
                 "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_table, span(rows, table_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the table");
+    SKM_REQUIRE(!overlap(d_table, span(rows, table_stride, d, size), d_out, span(n, out_stride, d, size)) &&
+                !overlap(d_ids, n * (ids_type == SKM_I64 ? 8 : 4), d_out, span(n, out_stride, d, size)), "out overlaps the table or the ids");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup");
     return for_type(type, [&](auto sample) {
@@ -369,6 +370,7 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
         SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps grad");
         SKM_REQUIRE(!d_grad_weights || !overlap(d_rows, span(n_rows, rows_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps the rows");
     }
+    SKM_REQUIRE(!overlap(d_weights, n * choices * weight_size, d_grad_weights, n * choices * weight_size), "grad_weights overlaps the weights");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/combine_grad");
     return for_type(type, [&](auto sample) {

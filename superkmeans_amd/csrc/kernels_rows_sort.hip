@@ -674,8 +674,10 @@ int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices,
     SKM_REQUIRE((address(d_choices) | address(d_slots) | address(d_order) | address(d_offsets)) % 4 == 0,
                 "pointers must be aligned to their elements");
     const size_t places = n * choices;
-    SKM_REQUIRE(!overlap(d_choices, places * 4, d_slots, places * 4) && !overlap(d_choices, places * 4, d_order, places * 4),
-                "slots and order must not overlap the choices");
+    SKM_REQUIRE(!overlap(d_choices, places * 4, d_slots, places * 4) && !overlap(d_choices, places * 4, d_order, places * 4) &&
+                !overlap(d_slots, places * 4, d_order, places * 4) && !overlap(d_slots, places * 4, d_offsets, (groups + 1) * 4) &&
+                !overlap(d_choices, places * 4, d_offsets, (groups + 1) * 4) && !overlap(d_order, places * 4, d_offsets, (groups + 1) * 4),
+                "choices, slots, order and offsets must not overlap");
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/route");
     if (places == 0) return skm_fill_u32(ctx, d_offsets, 0, groups + 1);

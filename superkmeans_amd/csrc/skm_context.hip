@@ -263,6 +263,21 @@ int skm_device_count(int* out_count) {
     return SKM_OK;
 }
 
+// Puts the calling thread's device back: a caller that brings its own stream has work of its own on some device.
+class DeviceAsItWas {
+  public:
+    explicit DeviceAsItWas(const bool put_back) : known_(put_back && hipGetDevice(&device_) == hipSuccess) {}
+    ~DeviceAsItWas() {
+        if (known_) (void) hipSetDevice(device_);
+    }
+    DeviceAsItWas(const DeviceAsItWas&) = delete;
+    DeviceAsItWas& operator=(const DeviceAsItWas&) = delete;
+
+  private:
+    int device_ = 0;
+    bool known_;
+};
+
 static int create_context(int device, bool own_stream, void* stream, skm_ctx** out_ctx) {
     if (!out_ctx) return set_error(SKM_ERR_INVALID, "skm_ctx_create: null output");
     *out_ctx = nullptr;
@@ -271,6 +286,7 @@ static int create_context(int device, bool own_stream, void* stream, skm_ctx** o
         return set_error(SKM_ERR_NO_DEVICE, "skm_ctx_create: no HIP device is visible");
     if (device < 0 || device >= n)
         return set_error(SKM_ERR_INVALID, "skm_ctx_create: device %d out of range [0,%d)", device, n);
+    const DeviceAsItWas as_it_was(!own_stream);
     SKM_HIP_TRY(hipSetDevice(device));
     hipDeviceProp_t prop;
     SKM_HIP_TRY(hipGetDeviceProperties(&prop, device));
@@ -312,6 +328,7 @@ int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx) {
 
 int skm_ctx_destroy(skm_ctx* ctx) {
     if (!ctx) return SKM_OK;
+    const DeviceAsItWas as_it_was(!ctx->owns_stream);
     // Teardown keeps going after a failure so that every resource gets its release call.
     (void) hipSetDevice(ctx->device);
     (void) hipStreamSynchronize(ctx->stream);

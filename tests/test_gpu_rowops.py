@@ -198,7 +198,8 @@ def spread_ids(g, n, rows, how):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("how", ["even", "one", "none", "two runs", "text"])
 @pytest.mark.parametrize("n,rows,d", [(1, 1, 1), (5, 3, 7), (63, 40, 8), (64, 1, 100), (257, 300, 130), (2048, 1000, 24),
-                                      (2049, 1000, 24), (2049, 3, 257), (5000, 70001, 8), (40000, 2049, 20)])
+                                      (2049, 1000, 24), (2049, 3, 257), (5000, 70001, 8), (40000, 2049, 20),
+                                      (3000, 1100000, 3), (140000, 500, 5)])
 def test_lookup_grad(dev, ops, kind, how, n, rows, d):
     g = np.random.default_rng(n + d)
     grad = typed(g.standard_normal((n, d)), kind)
@@ -222,6 +223,17 @@ def test_lookup_grad(dev, ops, kind, how, n, rows, d):
             ops.lookup_grad(on_device, where, out, scale=scale, accumulate=True)
             close(out, want + held, sizes + np.abs(held), most + 3)
             assert np.array_equal(out.host()[~touched], held[~touched])
+
+
+def test_lookup_grad_of_a_million_tokens(dev, ops):
+    """More tiles of the sort than one workgroup adds up, the longest chunks, and rows that thousands of chunks belong to."""
+    g = np.random.default_rng(0)
+    n, rows, d = 1100000, 40, 2
+    grad, ids = typed(g.standard_normal((n, d)), "float16"), spread_ids(g, n, rows, "text")
+    out = dev(np.full((rows, d), 5), "float32")
+    ops.lookup_grad(dev(grad, "float16"), dev(ids, "int32"), out)
+    want, sizes, most = summed(grad, ids, rows, 1.0)
+    close(out, want, sizes, most + 2)
 
 
 def test_lookup_grad_of_nothing(dev, ops):
@@ -281,7 +293,8 @@ def routed(choices, groups):
 
 
 SHAPES = [(1, 1, 1), (1, 8, 64), (3, 2, 5), (64, 8, 64), (171, 6, 1000), (512, 2, 1022), (512, 2, 1023), (1024, 8, 8), (1025, 8, 8),
-          (2000, 4, 1024), (5000, 3, 2047), (5000, 3, 2048), (4096, 2, 100000), (70000, 4, 33), (300000, 4, 7)]
+          (2000, 4, 1024), (5000, 3, 2047), (5000, 3, 2048), (4096, 2, 100000), (70000, 4, 33), (300000, 4, 7),
+          (3000, 1, 1048576)]
 
 
 @pytest.mark.parametrize("n,choices,groups", SHAPES)
@@ -481,7 +494,9 @@ def test_quantize_decides_at_the_borders_like_64_bits(dev, ops):
 
 
 PRODUCTS = [(1, 1, 1), (1, 5, 3), (2, 64, 64), (3, 17, 100), (16, 256, 128), (17, 130, 1000), (33, 1000, 272), (64, 64, 2048),
-            (100, 300, 516), (129, 257, 1040), (300, 520, 64), (1, 1024, 4096), (8, 2000, 1024), (512, 512, 512), (257, 1023, 769)]
+            (100, 300, 516), (129, 257, 1040), (300, 520, 64), (1, 1024, 4096), (8, 2000, 1024), (512, 512, 512), (257, 1023, 769),
+            (300, 64, 15), (5, 6, 16), (300, 300, 31), (70, 33, 129), (250, 2048, 80), (100, 2048, 144), (40, 1000, 96), (1000, 1000, 100), (1000, 2048, 160),
+            (2048, 2040, 176)]
 
 
 def product_of(a, a_scales, b, b_scales, bias):
@@ -507,6 +522,35 @@ def test_product(dev, ops, out_kind, m, n, k):
         assert out.margin_untouched()
 
 
+@pytest.mark.parametrize("out_kind", ["float32", "bfloat16"])
+def test_product_of_a_long_prompt(dev, ops, out_kind):
+    """Whole and partial tiles of the largest shape, with columns that end inside a stage."""
+    g = np.random.default_rng(9)
+    m, n, k = 4093, 4090, 1000
+    a, b = g.integers(-128, 128, (m, k)), g.integers(-128, 128, (n, k))
+    a_scales, b_scales = typed(g.random(m) * 0.01, "float32"), typed(g.random(n) * 0.01, "float32")
+    out = dev(np.full((m, n), 5), out_kind)
+    ops.product(dev(a, "int8"), dev(a_scales, "float32"), dev(b, "int8"), dev(b_scales, "float32"), out)
+    want, size = product_of(a, a_scales, b, b_scales, None)
+    close(out, want, size, 4)
+
+
+def test_product_with_rows_far_apart(capi, ctx, dev, ops):
+    """Rows of a 2^24 bytes apart: past the 32-bit offsets that the tiles' loads use."""
+    m, n, k, stride = 300, 300, 64, 1 << 24
+    g = np.random.default_rng(1)
+    a, b = g.integers(-128, 128, (m, k)).astype(np.int8), g.integers(-128, 128, (n, k))
+    memory = ctx.empty(m * stride, np.int8)
+    for i in range(m):
+        capi.check(ctx.lib.skm_upload(ctx.handle, memory.offset(i * stride), a[i].ctypes.data, k))
+    da = dev(np.zeros((1, 1)), "int8")
+    da.shape, da._stride, da.data_ptr = (m, k), (stride, 1), lambda: memory.ptr
+    ones, out = dev(np.ones(300), "float32"), dev(np.zeros((m, n)), "float32")
+    ops.product(da, ones, dev(b, "int8"), ones, out)
+    assert np.array_equal(out.host(), a.astype(np.float64) @ b.T)
+    memory.free()
+
+
 def test_product_of_the_largest_values(dev, ops):
     """131,071 products of -128 and -128 are 2^31 - 2^14: the sum does not wrap."""
     k = 131071
@@ -519,7 +563,8 @@ def test_product_of_the_largest_values(dev, ops):
 @pytest.mark.parametrize("m,n,k,sizes", [
     (1, 8, 16, [1]), (5, 17, 100, [0, 5, 0]), (60, 300, 64, [1, 0, 20, 3, 16, 17]), (500, 130, 256, [0, 129, 128, 1, 0, 200]),
     (64, 1024, 512, [1] * 64), (700, 257, 528, [350, 0, 350]), (3, 40, 33, [0, 0, 0]), (200, 96, 144, [2] * 100), (90, 64, 64, [33, 32, 25]),
-    (1500, 520, 320, [700, 0, 513, 256]),
+    (1500, 520, 320, [700, 0, 513, 256]), (300, 64, 32, [0] * 70 + [1] * 100 + [0] * 5000 + [100, 0, 64]), (2100, 2048, 64, [600, 500, 0, 1000]),
+    (1000, 600, 80, [9, 11, 0, 30] * 20),
 ])
 def test_product_of_groups(dev, ops, out_kind, m, n, k, sizes):
     g = np.random.default_rng(m + n)
@@ -843,6 +888,9 @@ def test_refusals_of_the_library(dev, ops, capi):
         "product groups": lambda: lib.skm_product_i8(h, p, 2, 8, p, p, 2, 8, 8, p, None, 0, 16, p, far, 0, 2),
         "product overlapping groups": lambda: lib.skm_product_i8(h, p, 2, 8, p, p, 2, 8, 8, p, None, 2, 8, p, far, 0, 2),
         "product in place": lambda: lib.skm_product_i8(h, p, 2, 8, p, far, 2, 8, 8, far, None, 0, 0, None, p, 0, 2),
+        "product over its scales": lambda: lib.skm_product_i8(h, p, 2, 8, far + 64, p, 2, 8, 8, p, None, 0, 0, None, far, 0, 32),
+        "route over its slots": lambda: lib.skm_route(h, p, 2, 2, 4, far, far, far + 64, None, 0),
+        "weights in place": lambda: lib.skm_combine_rows_grad(h, p, 0, 4, 4, 4, p, 4, 4, far, 1, far + 256, 0, None, 4, far + 256),
         "product out unaligned": lambda: lib.skm_product_i8(h, p, 2, 8, p, p, 2, 8, 8, p, None, 0, 0, None, far + 2, 0, 2),
     }
     for what, call in bad.items():
