@@ -168,15 +168,18 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
 
 // grad_rows[slot[t][j]] = w[t][j] * grad[t] and grad_w[t][j] = <grad[t], rows[slot[t][j]]>: one walk over the token's row
 // for each GRAD_CHOICES choices, WAVES wavefronts per token.
+template <int WAVES>
+constexpr int GRAD_THREADS = WAVES > 4 ? WAVES * 64 : ROWS_THREADS;
+
 template <class T, int E, int WAVES, int GRAD_CHOICES>
-__global__ __launch_bounds__(ROWS_THREADS) void combine_rows_grad_kernel(
+__global__ __launch_bounds__(GRAD_THREADS<WAVES>) void combine_rows_grad_kernel(
     const T* __restrict__ grad, const size_t n, const uint32_t vectors, const uint32_t last, const size_t grad_stride, const T* __restrict__ rows,
     const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const uint32_t choices,
     const void* __restrict__ weights, const int weights_type, T* __restrict__ grad_rows, const size_t grad_rows_stride,
     void* __restrict__ grad_weights
 ) {
-    constexpr int TOKENS = ROWS_THREADS / 64 / WAVES;  // tokens per workgroup
-    __shared__ float part[ROWS_THREADS / 64][GRAD_CHOICES];
+    constexpr int TOKENS = GRAD_THREADS<WAVES> / 64 / WAVES;  // tokens per workgroup
+    __shared__ float part[GRAD_THREADS<WAVES> / 64][GRAD_CHOICES];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint32_t in_row = threadIdx.x % (64 * WAVES);
     // every thread of a workgroup takes the same number of turns, so that all of them meet at the barriers
@@ -380,9 +383,10 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
             const uint32_t vectors = (uint32_t) ((d + E - 1) / E);
             const auto launch = [&](auto waves, auto together) {
                 constexpr int WAVES = decltype(waves)::value;
-                const size_t turns = (n + ROWS_THREADS / 64 / WAVES - 1) / (ROWS_THREADS / 64 / WAVES);
+                constexpr size_t TOKENS = GRAD_THREADS<WAVES> / 64 / WAVES;
+                const size_t turns = (n + TOKENS - 1) / TOKENS;
                 const unsigned blocks = (unsigned) std::min<uint64_t>(ROWS_MAX_BLOCKS, turns);
-                combine_rows_grad_kernel<T, E, WAVES, decltype(together)::value><<<blocks, ROWS_THREADS, 0, ctx->stream>>>(
+                combine_rows_grad_kernel<T, E, WAVES, decltype(together)::value><<<blocks, GRAD_THREADS<WAVES>, 0, ctx->stream>>>(
                     (const T*) d_grad, n, vectors, (uint32_t) (d - E), grad_stride, (const T*) d_rows, n_rows, rows_stride, d_slots, (uint32_t) choices,
                     d_weights, weights_type, (T*) d_grad_rows, grad_rows_stride, d_grad_weights);
                 return check_hip(hipGetLastError(), "combine_rows_grad_kernel launch");
@@ -392,6 +396,9 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
                 if (choices <= 4) return launch(waves, std::integral_constant<int, 4>{});
                 return launch(waves, std::integral_constant<int, 8>{});
             };
+            // few long rows: what a call takes is one walk over a row (9 rows of 3,968 over 6 choices 17 us with 4 wavefronts, 13 with
+            // 16; 300 rows of 4,096 over 8 choices 23 and 26)
+            if (vectors > 256 && n <= 64) return launch_waves(std::integral_constant<int, 16>{});
             if (vectors > 64) return launch_waves(std::integral_constant<int, 4>{});
             return launch_waves(std::integral_constant<int, 1>{});
         });

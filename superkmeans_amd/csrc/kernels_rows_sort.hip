@@ -483,10 +483,11 @@ __device__ __forceinline__ Crossing crossing_row(const GradArgs& g, const uint32
 // `alone_blocks` workgroups), a longer one a workgroup, whose wavefronts take contiguous shares, added in order: such rows
 // begin at least JOIN_ALONE chunks apart, so a workgroup looks for the one of JOIN_ALONE chunks.
 constexpr uint32_t JOIN_ALONE = 16;
+constexpr int JOIN_THREADS = 512;
 
 template <class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_join_kernel(const GradArgs g, const uint32_t alone_blocks) {
-    constexpr int WAVES = ROWS_THREADS / 64;
+__global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const GradArgs g, const uint32_t alone_blocks) {
+    constexpr int WAVES = JOIN_THREADS / 64;
     __shared__ vec_of<float, E> share[WAVES][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const size_t stride = (size_t) 2 * g.d;
@@ -641,7 +642,7 @@ struct GradPlan {
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
         // The additions of a chunk, and of a row's chunks, are chains: longer chunks for more tokens keep the second short
         // where many tokens are on one row.
-        chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 128 : 256;
+        chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 64 : 256;
         chunks = (uint32_t) ((n + chunk - 1) / chunk);
         at_parts = sort.bytes;
         bytes = at_parts + aligned((size_t) chunks * 2 * d * 4);
@@ -768,9 +769,10 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
                 return set_error(SKM_ERR_INVALID, "skm_lookup_rows_grad: too many rows for one launch");
             lookup_grad_kernel<T, O, E><<<(unsigned) blocks, ROWS_THREADS, 0, ctx->stream>>>(g, s, (uint32_t) chunk_blocks);
             SKM_TRY(check_hip(hipGetLastError(), "lookup_grad_kernel launch"));
-            const uint32_t alone_blocks = (uint32_t) (((uint64_t) g.chunks * g.pieces + PER_BLOCK - 1) / PER_BLOCK);
+            constexpr uint64_t JOINS = JOIN_THREADS / 64;
+            const uint32_t alone_blocks = (uint32_t) (((uint64_t) g.chunks * g.pieces + JOINS - 1) / JOINS);
             const uint32_t long_blocks = (g.chunks + JOIN_ALONE - 1) / JOIN_ALONE * g.pieces;
-            lookup_grad_join_kernel<O, E><<<alone_blocks + long_blocks, ROWS_THREADS, 0, ctx->stream>>>(g, alone_blocks);
+            lookup_grad_join_kernel<O, E><<<alone_blocks + long_blocks, JOIN_THREADS, 0, ctx->stream>>>(g, alone_blocks);
             return check_hip(hipGetLastError(), "lookup_grad_join_kernel launch");
         });
     };
