@@ -57,7 +57,8 @@ template <class T, int E>
 using bits_of = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> __attribute__((ext_vector_type(E)));
 
 // WAVES wavefronts to a row.  A row of up to 64 WAVES HELD vectors is read once and held in registers; of a longer one what is
-// past that is read twice.
+// past that is read twice.  Bound by memory for 32-bit rows (4,096 of 8,192 elements 29 us, 5.8 TB/s), by memory and the dozen
+// instructions per element about equally for 16-bit ones (8,192 of 4,096 24 us, 4.2 TB/s).
 constexpr int QUANTIZE_THREADS = 256;
 
 template <class T, int E, int WAVES, int HELD>
@@ -203,7 +204,8 @@ __device__ __forceinline__ intx4 load16_short(const int8_t* row, const int k, co
 // A workgroup owns 16 RT rows and 16 NB columns of the result; its wavefronts share the columns of the operands, and
 // their 32-bit sums are added through LDS (exact, so the split does not show).  With a row or a few per matrix every
 // byte of the weights is read once and used at once, so nothing is gained by LDS; what counts is how many bytes are on their
-// way: each wavefront requests AHEAD steps of 64 columns before it uses the first.
+// way: each wavefront requests AHEAD steps of 64 columns before it uses the first.  Bound by memory: 64 matrices of 2,048 x 1,024
+// on 512 rows take 30 us, 4.6 TB/s; one row through 4,096 x 4,096 5.7 us, 3 TB/s, where the launch and one latency are most of it.
 template <class O, int RT, int NB, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs p, const uint32_t tiles_n) {
     constexpr int TM = 16 * RT, TN = 16 * NB;
@@ -292,17 +294,21 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const Prod
 
 // ---- many rows: tiles through LDS ----
 //
-// Four wavefronts, each FM x FN blocks of 32 x 32, so a tile is 64 FM x 64 FN.  A stage is 128 columns (a cache line) of
-// both operands; two stages are in LDS and a third is on its way in registers.  A wavefront reads (FM + FN) KB of LDS for each
-// FM FN instructions: at 4 x 4 half of what the LDS can give in the time of the matrix instructions, at 2 x 4 (eight
-// wavefronts for the same tile) three quarters, and the stages' stores come on top.
-// Chunks of 16 bytes are stored at position chunk ^ (row % 8) of their row, so that the 32 rows of a block, 128 bytes
-// apart, are read from different banks.
+// 2 x WN wavefronts, each FM x FN blocks of 32 x 32, so a tile is 64 FM x 32 WN FN.  A stage is 128 columns (a cache line) of
+// both operands; two stages are in LDS and a third is on its way in registers.
+// The largest tile is 256 x 256 by eight wavefronts of 128 x 64.  Four of 128 x 128 read a third less LDS and hold 512 registers,
+// one wavefront to a SIMD: whatever it waits for, the matrix unit waits for too (8,192 x 8,192 x 4,096: 263 us against 253, and
+// 230 against 191 on zeros, where power does not limit the clock).  Two per SIMD fill each other's waits.
+// What bounds it: 253 us are 2.17 PFLOP/s of 8-bit operations, 43 % of the matrix units' peak.  Without the loads from memory it
+// takes 12 % less, with all stages reading the same columns 3 % less: it is neither memory nor the fabric, but the LDS
+// traffic next to the products, and on real data the clock, which falls with the bits that change.
+// Chunks of 16 bytes are stored at position chunk ^ (row / 2 % 8) of their row: two rows fill the banks once, so the 16 rows
+// that are read at a time have to differ in the pair, not in the row (row % 8 there: 2 % more time).
 constexpr int STAGE_K = 128;
 
-template <int FM, int FN>
+template <int FM, int FN, int WN>
 constexpr size_t tiles_lds_bytes() {
-    return (size_t) 2 * (64 * FM + 64 * FN) * STAGE_K;
+    return (size_t) 2 * (64 * FM + 32 * WN * FN) * STAGE_K;
 }
 
 // Number of a workgroup to tile: workgroups whose number is equal mod 8 run on the same die and share its L2, where 32 of them
@@ -322,9 +328,9 @@ struct TileMap {
     }
 };
 
-template <class O, int FM, int FN>
-__global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(const ProductArgs p, const TileMap map) {
-    constexpr int TM = 64 * FM, TN = 64 * FN, NLA = TM / 32, NLB = TN / 32;
+template <class O, int FM, int FN, int WN>
+__global__ __launch_bounds__(128 * WN, 2) void product_tiles_kernel(const ProductArgs p, const TileMap map) {
+    constexpr int TM = 64 * FM, TN = 32 * WN * FN, ROWS = 16 * WN, NLA = TM / ROWS, NLB = TN / ROWS;  // ROWS of a load by all threads
     constexpr uint32_t STAGE = (TM + TN) * STAGE_K;
     extern __shared__ __align__(16) int8_t lds[];  // [2][TM + TN][STAGE_K]
     uint32_t tile_m, tile_n;
@@ -333,7 +339,7 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     if (rows.first >= rows.end) return;
     const uint32_t n0 = tile_n * TN;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t wm = (wave >> 1) * FM * 32, wn = (wave & 1) * FN * 32;
+    const uint32_t wm = wave / WN * FM * 32, wn = wave % WN * FN * 32;
 
     // memory to registers: a thread takes 16 bytes of every 32nd row; rows past the end repeat the last one and are not stored
     const uint32_t ld_row = tid >> 3, ld_chunk = tid & 7;
@@ -341,9 +347,9 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     const int8_t* b_base = p.b + rows.group * p.b_group_stride + (size_t) n0 * p.b_stride;
     uint32_t a_at[NLA], b_at[NLB];
 #pragma unroll
-    for (int i = 0; i < NLA; ++i) a_at[i] = min(ld_row + 32 * i, rows.end - 1 - rows.first) * (uint32_t) p.a_stride + ld_chunk * 16;
+    for (int i = 0; i < NLA; ++i) a_at[i] = min(ld_row + ROWS * i, rows.end - 1 - rows.first) * (uint32_t) p.a_stride + ld_chunk * 16;
 #pragma unroll
-    for (int i = 0; i < NLB; ++i) b_at[i] = min(ld_row + 32 * i, p.n - 1 - n0) * (uint32_t) p.b_stride + ld_chunk * 16;
+    for (int i = 0; i < NLB; ++i) b_at[i] = min(ld_row + ROWS * i, p.n - 1 - n0) * (uint32_t) p.b_stride + ld_chunk * 16;
     intx4 ra[NLA], rb[NLB];
     const uint32_t stages = (p.k + STAGE_K - 1) / STAGE_K, full = p.k / STAGE_K;
     const auto request = [&](const uint32_t s) {
@@ -364,23 +370,23 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
         if (s < full) request(s);
         else request_last(s);
     };
-    const uint32_t st = ld_row * STAGE_K + ((ld_chunk ^ (ld_row & 7)) << 4);
+    const uint32_t st = ld_row * STAGE_K + ((ld_chunk ^ ((ld_row >> 1) & 7)) << 4);
     const auto publish = [&](const uint32_t buffer) {
         int8_t* to = lds + buffer * STAGE + st;
 #pragma unroll
-        for (int i = 0; i < NLA; ++i) *reinterpret_cast<intx4*>(to + i * 32 * STAGE_K) = ra[i];
+        for (int i = 0; i < NLA; ++i) *reinterpret_cast<intx4*>(to + i * ROWS * STAGE_K) = ra[i];
 #pragma unroll
-        for (int i = 0; i < NLB; ++i) *reinterpret_cast<intx4*>(to + (TM + i * 32) * STAGE_K) = rb[i];
+        for (int i = 0; i < NLB; ++i) *reinterpret_cast<intx4*>(to + (TM + i * ROWS) * STAGE_K) = rb[i];
     };
     // registers of a block: lane l holds row l % 32 and 16 columns from 16 (l / 32) on
     const uint32_t fr = (lane & 31) * STAGE_K;
     intx4 fa[2][FM], fb[2][FN];
     const auto fetch = [&](const uint32_t buffer, const int slice, const int to) {
-        const int8_t* at = lds + buffer * STAGE + fr + (((2 * slice + (lane >> 5)) ^ (lane & 7)) << 4);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const intx4*>(at + (wm + i * 32) * STAGE_K);
+        const int8_t* at = lds + buffer * STAGE + fr + (((2 * slice + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
 #pragma unroll
         for (int j = 0; j < FN; ++j) fb[to][j] = *reinterpret_cast<const intx4*>(at + (TM + wn + j * 32) * STAGE_K);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[to][i] = *reinterpret_cast<const intx4*>(at + (wm + i * 32) * STAGE_K);
     };
     intx16 acc[FM][FN] = {};
     const auto multiply = [&](const int of) {
@@ -393,16 +399,8 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     // One stage: while a slice is multiplied the next one is read, a read every second product; the barrier sits before the last
     // slice's products, when every read of the stage has returned, and the next stage's first slice is read under them.
     // (Left to itself the compiler reads a slice right before its products: 3 % more time.)
-    const auto interleave = [] {
-        if constexpr (FM * FN >= 2 * (FM + FN)) {
-#pragma unroll
-            for (int i = 0; i < FM + FN; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
-                __builtin_amdgcn_sched_group_barrier(0x008, FM * FN / (FM + FN), 0);  // matrix instructions
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
+    // One stage: while a slice is multiplied the next one is read; the barrier sits before the last slice's products, when every
+    // read of the stage has returned, and the next stage's first slice is read under them.
     const auto stage = [&](const uint32_t s, auto hot) {  // hot: stages s + 1 and s + 2 exist and are whole
         constexpr bool HOT = decltype(hot)::value;
         const uint32_t cur = s & 1;
@@ -411,17 +409,17 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
         else if (s + 2 < stages) request_any(s + 2);
         fetch(cur, 1, 1);
         multiply(0);
-        interleave();
+        __builtin_amdgcn_sched_barrier(0);
         fetch(cur, 2, 0);
         multiply(1);
-        interleave();
+        __builtin_amdgcn_sched_barrier(0);
         fetch(cur, 3, 1);
         multiply(0);
-        interleave();
+        __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
         if (HOT || s + 1 < stages) fetch(cur ^ 1, 0, 0);
         multiply(1);
-        interleave();
+        __builtin_amdgcn_sched_barrier(0);
     };
     request_any(0);
     publish(0);
@@ -436,10 +434,10 @@ __global__ __launch_bounds__(256, FM == 4 ? 1 : 2) void product_tiles_kernel(con
     // Results, 32 rows at a time through LDS (each wavefront in a part of its own), so that rows are stored 16 bytes per lane.
     // Element r of block (i, j): row l % 32, column 8 (r / 4) + 4 (l / 32) + r % 4.
     constexpr int E = 16 / sizeof(O), COLUMNS = FN * 32, LD = COLUMNS + E;
-    static_assert((size_t) 4 * 32 * LD * sizeof(O) + 2 * TN * sizeof(float) <= (size_t) 2 * STAGE, "results go through the stages' LDS");
+    static_assert((size_t) 2 * WN * 32 * LD * sizeof(O) + 2 * TN * sizeof(float) <= (size_t) 2 * STAGE, "results go through the stages' LDS");
     __syncthreads();
     O* staged = reinterpret_cast<O*>(lds) + wave * 32 * LD;
-    float* b_scale = reinterpret_cast<float*>(lds + (size_t) 4 * 32 * LD * sizeof(O));
+    float* b_scale = reinterpret_cast<float*>(lds + (size_t) 2 * WN * 32 * LD * sizeof(O));
     float* bias = b_scale + TN;
     if (tid < TN) {
         const size_t n = (size_t) rows.group * p.n + min(n0 + tid, p.n - 1);
@@ -491,10 +489,11 @@ int launch_few_rows(skm_ctx* ctx, const ProductArgs& p) {
     return check_hip(hipGetLastError(), "product_few_rows_kernel launch");
 }
 
-template <class O, int FM, int FN>
+template <class O, int FM, int FN, int WN>
 int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
-    constexpr size_t lds = tiles_lds_bytes<FM, FN>();
-    const uint32_t tiles_n = (p.n + 64 * FN - 1) / (64 * FN);
+    constexpr size_t lds = tiles_lds_bytes<FM, FN, WN>();
+    constexpr uint32_t TN = 32 * WN * FN;
+    const uint32_t tiles_n = (p.n + TN - 1) / TN;
     const uint64_t tiles_m = (uint64_t) (p.m + 64 * FM - 1) / (64 * FM) + (p.offsets ? p.groups : 0);
     uint32_t super_n = 1;
     while (super_n < 8 && super_n < tiles_n) super_n *= 2;
@@ -505,26 +504,30 @@ int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
     const auto launch = [&](auto kernel) {
         SKM_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds),
                           "hipFuncSetAttribute(MaxDynamicSharedMemorySize)"));
-        kernel<<<(unsigned) blocks, 256, lds, ctx->stream>>>(p, map);
+        kernel<<<(unsigned) blocks, 128 * WN, lds, ctx->stream>>>(p, map);
         return check_hip(hipGetLastError(), "product_tiles_kernel launch");
     };
-    return launch(product_tiles_kernel<O, FM, FN>);
+    return launch(product_tiles_kernel<O, FM, FN, WN>);
 }
 
-// The kernel for a call: the largest tile that still gives every compute unit a workgroup.  A larger tile reads each operand
-// fewer times, and loses more than that where it leaves compute units without one (us, bf16 results):
-//     rows x n x k          256 x 256  128 x 128  128 x 64  64 x 64    few rows: 32 x 64  32 x 32  32 x 16  16 x 16
-//     8192 x 8192 x 4096       287        333        412      507
-//     1024 x 4096 x 4096        72         30         34       37
-//      512 x 4096 x 4096                   27         19       20                   50
-//      256 x 4096 x 4096                   24         18       15                   26
-//      128 x 4096 x 4096                              18       15                   14       17
-//       64 x 4096 x 4096                                       15                   14       10       12       12
-//       64 x 1024 x 4096                                                                     10        8        7
-//        1 x 4096 x 4096                                                                      8        7        7
-// Over groups the host knows the rows of a group on average only.  There 64 x 64 tiles pay from 9 rows on (64 groups, n 2048,
-// k 1024: 16 rows each 27 us against 36 us with few rows' kernel, 8 rows each 27 with 16 x 64 of it and more with tiles), and the
-// 256 x 256 tiles never, as the groups' ends leave half a tile each (8 groups, 32768 x 4096 x 1536: 294 against 307 us).
+// The kernel for a call: the largest tile that still gives every compute unit a workgroup (the largest one already where three
+// quarters get one).  A larger tile reads each operand fewer times, and loses more than that where it leaves compute units
+// without one (us, bf16 results, the chosen one in brackets):
+//     rows x n x k         256 x 256  128 x 256  128 x 128  128 x 64  64 x 64   few rows: 32 x 64  32 x 32  32 x 16  16 x 16
+//     8192 x 8192 x 4096     [258]       292        320       380
+//     3000 x 4096 x 4096      [55]        67         63        77        89
+//     2048 x 4096 x 4096       49        [38]        43        51
+//     1024 x 4096 x 4096                  30        [24]       28        32
+//      512 x 4096 x 4096                  29         21       [19]       19                  50
+//      256 x 4096 x 4096                             20        17       [15]                 26
+//      128 x 4096 x 4096                                       17        14                 [14]       17
+//       64 x 4096 x 4096                                                                     14       [10]       12
+//       64 x 1024 x 4096                                                                               10         8       [7]
+//       16 x 4096 x 4096                                                                                9         7       [8]
+// Over groups the host knows the rows of a group on average only, and every group's last tile is part empty.  There 64 x 64
+// tiles pay from 9 rows on (64 groups, n 2048, k 1024: 16 rows each 29 us against 35 us with the few rows' best tile, 8 rows
+// each 29 us with 16 x 64 of those), 128 rows to a tile from 49 on (64 rows each 36 against 40 us), 256 from 129 on
+// (512 rows each 125 us with either; 8 groups of 4,096, n 4096, k 1536: 267 against 278 us).
 template <class O>
 int launch_product(skm_ctx* ctx, const ProductArgs& p) {
     constexpr uint64_t WANTED = 256;
@@ -533,15 +536,12 @@ int launch_product(skm_ctx* ctx, const ProductArgs& p) {
     const auto tiles = [&](const uint64_t tm, const uint64_t tn) { return p.groups * ((rows + tm - 1) / tm) * ((p.n + tn - 1) / tn); };
     // what the tiles' loads assume: 16 columns at least, a tile's offsets in 32 bits
     if (p.k >= 16 && p.a_stride < (1u << 23) && p.b_stride < (1u << 23)) {
-        // The large tiles run one to a compute unit, so a last round that is partly filled takes as long as a full one; the medium
-        // ones run two to a unit and drift apart.  Microseconds of a round by the columns, from products of whole rounds.
-        const double columns = p.k / 1024.0;
-        const double large = (double) ((tiles(256, 256) + 255) / 256) * (10.0 + 15.0 * columns);
-        const double medium = std::max(1.0, tiles(128, 128) / 512.0 + 0.25) * (4.0 + 9.4 * columns);
-        if (!grouped && tiles(256, 256) >= WANTED && large <= medium) return launch_tiles<O, 4, 4>(ctx, p);
-        if (rows > 64 && tiles(128, 128) >= WANTED) return launch_tiles<O, 2, 2>(ctx, p);
-        if (rows > 64 && tiles(128, 64) >= WANTED) return launch_tiles<O, 2, 1>(ctx, p);
-        if (rows > (grouped ? 8 : 32) && tiles(64, 64) >= WANTED) return launch_tiles<O, 1, 1>(ctx, p);
+        const uint64_t many = grouped ? 48 : 64;
+        if (rows > 128 && tiles(256, 256) >= WANTED * 3 / 4) return launch_tiles<O, 4, 2, 4>(ctx, p);
+        if (rows > many && tiles(128, 256) >= WANTED) return launch_tiles<O, 2, 2, 4>(ctx, p);
+        if (rows > many && tiles(128, 128) >= WANTED) return launch_tiles<O, 2, 1, 4>(ctx, p);
+        if (rows > many && tiles(128, 64) >= WANTED) return launch_tiles<O, 2, 1, 2>(ctx, p);
+        if (rows > (grouped ? 8 : 32) && tiles(64, 64) >= WANTED) return launch_tiles<O, 1, 1, 2>(ctx, p);
     }
     if (rows > 16 && tiles(32, 64) >= WANTED) return launch_few_rows<O, 2, 4, 8, 2>(ctx, p);
     if (rows > 16 && tiles(32, 32) >= WANTED) return launch_few_rows<O, 2, 2, 8, 4>(ctx, p);

@@ -38,7 +38,8 @@ __device__ __forceinline__ uint64_t id_at(const void* ids, const int ids_type, c
 
 // out[t] = scale * table[id_t], a row of zeros where the id is no row.  A wavefront takes TOKENS rows at a time and requests all
 // their ids, then UNROLL vectors per lane of all the rows, before it stores the first: with one row at a time the wavefronts
-// that a compute unit holds do not have enough bytes on their way.
+// that a compute unit holds do not have enough bytes on their way (a million rows of 4 KiB: one row at a time 790 us, four 782,
+// eight 783).  Bound by the stores: those 4.1 GB in 783 us are 5.2 TB/s next to as much read from the memory-side cache.
 template <class T, int E, int TOKENS>
 __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
     const T* __restrict__ table, const size_t rows, const size_t table_stride, const void* __restrict__ ids, const int ids_type,
@@ -76,7 +77,8 @@ __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
     }
 }
 
-// out[slot[t][j]] = x[t] for every choice j that has a slot: the row is read once and stored once per choice.
+// out[slot[t][j]] = x[t] for every choice j that has a slot: the row is read once and stored once per choice.  Bound by memory:
+// 32,768 rows of 8 KiB to 2 groups each, 0.8 GB, in 134 us, 6.0 TB/s.
 template <class T, int E>
 __global__ __launch_bounds__(ROWS_THREADS) void dispatch_rows_kernel(
     const T* __restrict__ x, const size_t x_stride, const size_t n, const uint32_t* __restrict__ slots, const uint32_t choices,
@@ -120,7 +122,8 @@ __device__ __forceinline__ void put_weight(void* weights, const int type, const 
 constexpr int COMBINE_UNROLL = 4;  // vectors per lane
 constexpr int COMBINE_AHEAD = 2;   // choices whose rows are requested together
 
-// out[t] = sum_j w[t][j] * rows[slot[t][j]], j ascending, in fp32.
+// out[t] = sum_j w[t][j] * rows[slot[t][j]], j ascending, in fp32.  A lane has COMBINE_AHEAD x COMBINE_UNROLL vectors on their
+// way.  Bound by memory: 16,384 sums over 8 rows of 3 KiB, 0.45 GB, in 75 us, 6.0 TB/s.
 template <class T, int E>
 __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
     const T* __restrict__ rows, const size_t n_rows, const size_t rows_stride, const uint32_t* __restrict__ slots, const size_t n,
@@ -167,7 +170,8 @@ __global__ __launch_bounds__(ROWS_THREADS) void combine_rows_kernel(
 }
 
 // grad_rows[slot[t][j]] = w[t][j] * grad[t] and grad_w[t][j] = <grad[t], rows[slot[t][j]]>: one walk over the token's row
-// for each GRAD_CHOICES choices, WAVES wavefronts per token.
+// for each GRAD_CHOICES choices, WAVES wavefronts per token.  Bound by memory: 10,007 tokens of 4,000 bytes and 4 choices,
+// 0.36 GB, in 68 us, 5.3 TB/s (85 us with one wavefront per token, which has a token's vectors in four turns).
 template <int WAVES>
 constexpr int GRAD_THREADS = WAVES > 4 ? WAVES * 64 : ROWS_THREADS;
 

