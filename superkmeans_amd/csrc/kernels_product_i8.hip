@@ -341,7 +341,7 @@ __global__ __launch_bounds__(128 * WN, 2) void product_tiles_kernel(const Produc
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t wm = wave / WN * FM * 32, wn = wave % WN * FN * 32;
 
-    // memory to registers: a thread takes 16 bytes of every 32nd row; rows past the end repeat the last one and are not stored
+    // memory to registers: a thread takes 16 bytes of every ROWS-th row; rows past the end repeat the last one and are not stored
     const uint32_t ld_row = tid >> 3, ld_chunk = tid & 7;
     const int8_t* a_base = p.a + (size_t) rows.first * p.a_stride;
     const int8_t* b_base = p.b + rows.group * p.b_group_stride + (size_t) n0 * p.b_stride;
@@ -396,9 +396,6 @@ __global__ __launch_bounds__(128 * WN, 2) void product_tiles_kernel(const Produc
             for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[of][j], fa[of][i], acc[i][j], 0, 0, 0);
     };
 
-    // One stage: while a slice is multiplied the next one is read, a read every second product; the barrier sits before the last
-    // slice's products, when every read of the stage has returned, and the next stage's first slice is read under them.
-    // (Left to itself the compiler reads a slice right before its products: 3 % more time.)
     // One stage: while a slice is multiplied the next one is read; the barrier sits before the last slice's products, when every
     // read of the stage has returned, and the next stage's first slice is read under them.
     const auto stage = [&](const uint32_t s, auto hot) {  // hot: stages s + 1 and s + 2 exist and are whole

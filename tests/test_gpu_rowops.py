@@ -598,6 +598,20 @@ def test_offsets_past_the_rows_are_clamped(dev, ops):
             assert np.all(out.host()[row] == value * 32)
 
 
+def test_groups_that_begin_behind_the_first_row(dev, ops):
+    """A part of a larger table of offsets: rows before its first group and behind its last one are nobody's."""
+    g = np.random.default_rng(4)
+    m, n, k, offsets = 700, 300, 64, [5, 5, 90, 91, 600]
+    a, b = g.integers(-128, 128, (m, k)), g.integers(-128, 128, (4, n, k))
+    ones, out = dev(np.ones(m), "float32"), dev(np.full((m, n), 5), "float32")
+    ops.product(dev(a, "int8"), ones, dev(b, "int8"), dev(np.ones((4, n)), "float32"), out, offsets=dev(offsets, "int32"))
+    want = np.full((m, n), 5.0)
+    for e in range(4):
+        rows = slice(offsets[e], offsets[e + 1])
+        want[rows] = a[rows].astype(np.float64) @ b[e].T
+    assert np.array_equal(out.host(), want)
+
+
 def test_products_of_rows_that_hold_nan_are_nan(dev, ops):
     x = np.ones((3, 64))
     x[1, 5], x[2, 0] = np.nan, -np.inf
@@ -605,6 +619,36 @@ def test_products_of_rows_that_hold_nan_are_nan(dev, ops):
     ops.quantize(dev(x, "float32"), q, s)
     ops.product(q, s, dev(np.ones((8, 64)), "int8"), dev(np.ones(8), "float32"), out)
     assert np.allclose(out.host()[0], 64, rtol=4 * U) and np.all(np.isnan(out.host()[1:]))
+
+
+@pytest.mark.parametrize("d", [1048573, 131072])
+def test_the_longest_rows(dev, ops, d):
+    g = np.random.default_rng(d)
+    table = typed(g.standard_normal((3, d)), "bfloat16")
+    ids, slots = np.array([2, -1, 0, 2]), np.array([[1, 2], [-1, 0], [3, -1], [-1, -1]])
+    x, rows, out = dev(np.zeros((4, d)), "bfloat16"), dev(np.zeros((4, d)), "bfloat16"), dev(np.zeros((4, d)), "bfloat16")
+    ops.lookup(dev(table, "bfloat16"), dev(ids, "int64"), x)
+    want = np.where((ids >= 0)[:, None], table[ids.clip(0)], 0)
+    assert np.array_equal(x.host(), want)
+    ds, weights = dev(slots, "int32"), typed(g.random((4, 2)), "float32")
+    ops.dispatch(x, ds, rows)
+    places = want[[1, 0, 0, 2]]
+    assert np.array_equal(rows.host(), places)
+    ops.combine(rows, ds, out, weights=dev(weights, "float32"))
+    picked = np.where((slots >= 0)[..., None], places[slots.clip(0)], 0)
+    parts = picked * weights[..., None]
+    close(out, parts.sum(1), np.abs(parts).sum(1), 3)
+    dots = dev(np.zeros((4, 2)), "float32")
+    ops.combine_grad(x, rows, ds, dev(weights, "float32"), None, dots)
+    products = picked * want[:, None]
+    close(dots, products.sum(-1), np.abs(products).sum(-1), d)
+    grad = dev(np.zeros((3, d)), "float32")
+    ops.lookup_grad(x, dev(ids, "int64"), grad)
+    sums, sizes, most = summed(want, ids, 3, 1.0)
+    close(grad, sums, sizes, most + 2)
+    q, scales = dev(np.zeros((4, d)), "int8"), dev(np.zeros(4), "float32")
+    ops.quantize(x, q, scales)
+    assert np.array_equal(q.raw(), steps(want)[0])
 
 
 # ---------------------------------------------------------------------------------------------------------------------
