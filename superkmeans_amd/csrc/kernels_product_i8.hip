@@ -299,9 +299,9 @@ __global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const Prod
 // The largest tile is 256 x 256 by eight wavefronts of 128 x 64.  Four of 128 x 128 read a third less LDS and hold 512 registers,
 // one wavefront to a SIMD: whatever it waits for, the matrix unit waits for too (8,192 x 8,192 x 4,096: 263 us against 253, and
 // 230 against 191 on zeros, where power does not limit the clock).  Two per SIMD fill each other's waits.
-// What bounds it: 253 us are 2.17 PFLOP/s of 8-bit operations, 43 % of the matrix units' peak.  Without the loads from memory it
-// takes 12 % less, with all stages reading the same columns 3 % less: it is neither memory nor the fabric, but the LDS
-// traffic next to the products, and on real data the clock, which falls with the bits that change.
+// What bounds it: 253 us are 2.17 PFLOP/s of 8-bit operations, 43 % of the matrix units' peak at 2.4 GHz.  By the counters the
+// units are busy in 55 % of the cycles, and there are 1.9 GHz of them: the clock falls with the bits that change in the
+// operands.  Memory is not it (0.4 GB past the L2; with every stage reading the same columns 3 % less time).
 // Chunks of 16 bytes are stored at position chunk ^ (row / 2 % 8) of their row: two rows fill the banks once, so the 16 rows
 // that are read at a time have to differ in the pair, not in the row (row % 8 there: 2 % more time).
 constexpr int STAGE_K = 128;

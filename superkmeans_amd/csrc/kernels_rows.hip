@@ -39,7 +39,8 @@ __device__ __forceinline__ uint64_t id_at(const void* ids, const int ids_type, c
 // out[t] = scale * table[id_t], a row of zeros where the id is no row.  A wavefront takes TOKENS rows at a time and requests all
 // their ids, then UNROLL vectors per lane of all the rows, before it stores the first: with one row at a time the wavefronts
 // that a compute unit holds do not have enough bytes on their way (a million rows of 4 KiB: one row at a time 790 us, four 782,
-// eight 783).  Bound by the stores: those 4.1 GB in 783 us are 5.2 TB/s next to as much read from the memory-side cache.
+// eight 783).  Bound by the stores: those 4.1 GB in 783 us are 5.2 TB/s, next to 1.5 GB of table rows
+// that miss the compute dies' L2.
 template <class T, int E, int TOKENS>
 __global__ __launch_bounds__(ROWS_THREADS) void lookup_rows_kernel(
     const T* __restrict__ table, const size_t rows, const size_t table_stride, const void* __restrict__ ids, const int ids_type,
