@@ -162,6 +162,8 @@ class RowOperators:
     def _scratch(self, scratch):
         if scratch is None:
             return None, 0
+        if not hasattr(scratch, "dtype"):
+            raise TypeError(f"scratch must be a device tensor, not {type(scratch).__name__}")
         name = _dtype_name(scratch.dtype)
         if name not in _SIZES:
             raise TypeError(f"scratch cannot be of {name}")

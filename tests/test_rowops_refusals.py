@@ -81,6 +81,7 @@ BAD = {
     "gradient between half types": lambda o: o.lookup_grad(T((3, 4), "bfloat16"), I((3,)), T((9, 4), "float16")),
     "gradient of other columns": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 5))),
     "gradient with a matrix of scratch": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 4)), scratch=T((9, 9))),
+    "gradient with a number for scratch": lambda o: o.lookup_grad(T((3, 4)), I((3,)), T((9, 4)), scratch=4096),
     "route of 64-bit choices": lambda o: o.route(Tensor((3, 2), "int64"), 4, I((3, 2)), I((5,))),
     "route slots of another shape": lambda o: o.route(I((3, 2)), 4, I((2, 3)), I((5,))),
     "route too few offsets": lambda o: o.route(I((3, 2)), 4, I((3, 2)), I((4,))),
