@@ -399,10 +399,8 @@ __device__ __forceinline__ void grad_of_chunk(const GradArgs& g, const RowSplit&
 #pragma unroll
         for (int q = 0; q < GRAD_AHEAD; ++q)
 #pragma unroll
-            for (int i = 0; i < GRAD_VECTORS; ++i) {
-                const uint32_t at = first + i * s.lanes;
-                if (at < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) token[q] * g.grad_stride + column<E>(at, g.last));
-            }
+            for (int i = 0; i < GRAD_VECTORS; ++i)  // past the row's end its last vector, which is not used: no conditions on loads
+                v[q][i] = load_vec<T, E>(grad + (size_t) token[q] * g.grad_stride + column<E>(min(first + i * s.lanes, g.vectors - 1), g.last));
 #pragma unroll
         for (int q = 0; q < GRAD_AHEAD; ++q) {
             if (j + q >= to) break;
@@ -412,8 +410,7 @@ __device__ __forceinline__ void grad_of_chunk(const GradArgs& g, const RowSplit&
                 if (row >= g.rows) return;
             }
 #pragma unroll
-            for (int i = 0; i < GRAD_VECTORS; ++i)
-                if (first + i * s.lanes < g.vectors) sum[i] += widen<E>(v[q][i]);
+            for (int i = 0; i < GRAD_VECTORS; ++i) sum[i] += widen<E>(v[q][i]);
         }
     }
     put(!goes_on);
@@ -534,17 +531,21 @@ __global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const Gr
         put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + column<E>(at, g.last), sum, g.scale, g.accumulate);
 }
 
-// Few tokens: one launch and no sort, 9 us for 1,021 tokens of 3 KiB into 4,096 rows (the sorted path takes six launches).  A workgroup owns every `step`-th row, reads all ids, and lists the tokens of its rows in order
+// Few tokens: one launch and no sort, 8 us for 1,021 tokens of 3 KiB into 4,096 rows (the sorted path takes six launches).  A workgroup owns a piece of every `step`-th row, reads all ids, and lists the tokens of its rows in order
 // (every wavefront those of a contiguous share).  Then its wavefronts take the rows one by one, and together those of
 // many tokens, each wavefront the tokens of its share.
 constexpr size_t FEW_TOKENS = 2048;
 constexpr int FEW_THREADS = 512, FEW_AHEAD = 4;
 constexpr uint32_t FEW_ROWS = 64;  // of a workgroup, at most
 constexpr uint32_t FEW_MOST = 8;   // tokens of a row that one wavefront adds up
+// A row's tokens are a chain here: with many on every row the sort is faster (2,048 tokens on one row: 71 us here, 16 sorted).
+inline bool few_tokens(const size_t n, const size_t rows) { return n <= FEW_TOKENS && (n <= 256 || n <= 32 * rows); }
+template <int E>
+constexpr int FEW_VECTORS = E >= 8 ? 2 : 4;  // vectors a lane holds of a row, at most
 
-template <class T, class O, int E>
+template <class T, class O, int E, int V>  // V: vectors a lane holds of a row
 __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const GradArgs g, const KeySource source, const uint32_t step) {
-    constexpr int WAVES = FEW_THREADS / 64, SHARE = FEW_TOKENS / WAVES, V = E >= 8 ? 2 : 4;  // V: vectors a lane holds of a row
+    constexpr int WAVES = FEW_THREADS / 64, SHARE = FEW_TOKENS / WAVES;
     __shared__ uint32_t listed[WAVES][SHARE];  // number of the row, token
     __shared__ uint32_t many[WAVES], of_row[FEW_ROWS];
     __shared__ vec_of<float, E> share[WAVES][V][64];
@@ -579,24 +580,24 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
             const uint32_t entry = k0 + lane < many[w] ? listed[w][k0 + lane] : 0xffffffffu;
             unsigned long long same = __ballot(entry >> 16 == r);
             while (same) {
+                // past the row's end its last vector, which is not used: conditions of lanes would keep the loads from being
+                // on their way together
                 vec_of<T, E> v[FEW_AHEAD][V];
-                int taken = 0;
+                const int taken = min(__popcll(same), FEW_AHEAD);
 #pragma unroll
-                for (int q = 0; q < FEW_AHEAD; ++q) {
-                    if (same) {
-                        const uint32_t t = __builtin_amdgcn_readlane(entry, __builtin_ctzll(same)) & 0xffffu;
+                for (int q = 0; q < FEW_AHEAD; ++q)
+                    if (q < taken) {
+                        const uint32_t t = __builtin_amdgcn_readlane(entry, (uint32_t) __builtin_ctzll(same)) & 0xffffu;
                         same &= same - 1;
 #pragma unroll
                         for (int i = 0; i < V; ++i)
-                            if (at + i * 64 < g.vectors) v[q][i] = load_vec<T, E>(grad + (size_t) t * g.grad_stride + column<E>(at + i * 64, g.last));
-                        taken = q + 1;
+                            v[q][i] = load_vec<T, E>(grad + (size_t) t * g.grad_stride + column<E>(min(at + i * 64, g.vectors - 1), g.last));
                     }
-                }
 #pragma unroll
                 for (int q = 0; q < FEW_AHEAD; ++q)
+                    if (q < taken)
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (q < taken && at + i * 64 < g.vectors) sum[i] += widen<E>(v[q][i]);
+                        for (int i = 0; i < V; ++i) sum[i] += widen<E>(v[q][i]);
             }
         }
     };
@@ -606,9 +607,9 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
         for (int i = 0; i < V; ++i)
             if (at + i * 64 < g.vectors) put_sum<O, E>(out + column<E>(at + i * 64, g.last), sum[i], g.scale, g.accumulate);
     };
-    const uint32_t pieces = (g.vectors + 64 * V - 1) / (64 * V);
-    for (uint32_t u = wave; u < mine * pieces; u += WAVES) {
-        const uint32_t r = u / pieces, at = u % pieces * (64 * V) + lane, tokens = of_row[r];
+    const uint32_t at = blockIdx.y * (64 * V) + lane;  // the workgroup's piece of the rows
+    for (uint32_t r = wave; r < mine; r += WAVES) {
+        const uint32_t tokens = of_row[r];
         if (tokens > FEW_MOST || (g.accumulate && tokens == 0)) continue;
         vec_of<float, E> sum[V] = {};
         if (tokens)
@@ -617,21 +618,18 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
     }
     for (uint32_t r = 0; r < mine; ++r) {
         if (of_row[r] <= FEW_MOST) continue;
-        for (uint32_t piece = 0; piece < pieces; ++piece) {
-            const uint32_t at = piece * (64 * V) + lane;
-            vec_of<float, E> sum[V] = {};
-            add_share(wave, r, at, sum);
+        vec_of<float, E> sum[V] = {};
+        add_share(wave, r, at, sum);
 #pragma unroll
-            for (int i = 0; i < V; ++i) share[wave][i][lane] = sum[i];
-            __syncthreads();
-            if (wave == 0) {
-                for (int w = 1; w < WAVES; ++w)
+        for (int i = 0; i < V; ++i) share[wave][i][lane] = sum[i];
+        __syncthreads();
+        if (wave == 0) {
+            for (int w = 1; w < WAVES; ++w)
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sum[i] += share[w][i][lane];
-                put(r, at, sum);
-            }
-            __syncthreads();
+                for (int i = 0; i < V; ++i) sum[i] += share[w][i][lane];
+            put(r, at, sum);
         }
+        __syncthreads();
     }
 }
 
@@ -642,7 +640,7 @@ struct GradPlan {
     size_t at_parts, bytes;
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
         // The additions of a chunk, and of a row's chunks, are chains: short chunks give more wavefronts and more sums to join
-        // (the whole call for 65,536 tokens of text: chunks of 16 160 us, of 32 168), longer ones for more tokens keep the joins
+        // (the whole call for 65,536 tokens of text: chunks of 16 160 us, of 32 168, before loads lost their conditions), longer ones for more tokens keep the joins
         // short where many are on one row (500,000 tokens on 4 rows: 32 247 us, 64 170, 128 149; a million of text: 32 173, 64
         // 163, 128 185).
         chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 64 : 256;
@@ -704,7 +702,7 @@ int skm_lookup_rows_grad_scratch(size_t n, size_t rows, size_t d, size_t* out_by
     SKM_REQUIRE(out_bytes, "null output");
     SKM_REQUIRE(d > 0 && d <= SKM_ROW_MAX_D, "d out of range");
     SKM_REQUIRE(rows < SKM_NO_ROW && n <= SKM_ROUTE_MAX_PLACES, "rows or n out of range");
-    *out_bytes = n <= FEW_TOKENS || rows == 0 ? 0 : GradPlan(n, rows, d).bytes;
+    *out_bytes = few_tokens(n, rows) || rows == 0 ? 0 : GradPlan(n, rows, d).bytes;
     return SKM_OK;
 }
 
@@ -747,11 +745,19 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
             g.vectors = (uint32_t) ((d + E - 1) / E);
             g.last = (uint32_t) (d - E);
             g.pieces = (g.vectors + 63) / 64;
-            if (n <= FEW_TOKENS) {
+            if (few_tokens(n, rows)) {
                 // a workgroup per row up to 1,024, then a few rows each: reading the ids costs a workgroup about as much as two rows
                 const uint32_t step = (uint32_t) std::max<size_t>(std::min<size_t>(rows, 1024), (rows + FEW_ROWS - 1) / FEW_ROWS);
-                lookup_grad_few_kernel<T, O, E><<<step, FEW_THREADS, 0, ctx->stream>>>(g, source, step);
-                return check_hip(hipGetLastError(), "lookup_grad_few_kernel launch");
+                const auto launch = [&](auto held) {
+                    constexpr int V = decltype(held)::value;
+                    const uint32_t pieces = (g.vectors + 64 * V - 1) / (64 * V);
+                    lookup_grad_few_kernel<T, O, E, V><<<dim3(step, pieces), FEW_THREADS, 0, ctx->stream>>>(g, source, step);
+                    return check_hip(hipGetLastError(), "lookup_grad_few_kernel launch");
+                };
+                if (g.vectors <= 64) return launch(std::integral_constant<int, 1>{});
+                if (g.vectors <= 128) return launch(std::integral_constant<int, 2>{});
+                if (FEW_VECTORS<E> > 2 && g.vectors <= 192) return launch(std::integral_constant<int, FEW_VECTORS<E> - 1>{});
+                return launch(std::integral_constant<int, FEW_VECTORS<E>>{});
             }
             const GradPlan plan(n, rows, d);
             void* at = nullptr;
