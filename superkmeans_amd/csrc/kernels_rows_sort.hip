@@ -440,7 +440,7 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit
 }
 
 // One launch for both: the chunks, whose wavefronts wait for memory, under the fill.  Bound by memory: 65,536 tokens of 1,536
-// 16-bit elements into 65,536 rows of fp32, 0.6 GB, in 121 us, 5.0 TB/s.
+// 16-bit elements into 65,536 rows of fp32, 0.6 GB, in 119 us, 5.1 TB/s.
 template <class T, class O, int E>
 __global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_kernel(const GradArgs g, const RowSplit s, const uint32_t chunk_blocks) {
     const uint32_t wave = threadIdx.x >> 6;
@@ -531,7 +531,8 @@ __global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const Gr
         put_sum<O, E>(reinterpret_cast<O*>(g.out) + (size_t) x.row * g.out_stride + column<E>(at, g.last), sum, g.scale, g.accumulate);
 }
 
-// Few tokens: one launch and no sort, 8 us for 1,021 tokens of 3 KiB into 4,096 rows (the sorted path takes six launches).  A workgroup owns a piece of every `step`-th row, reads all ids, and lists the tokens of its rows in order
+// Few tokens: one launch and no sort, 8 us for 1,021 tokens of 3 KiB into 4,096 rows (the sorted path takes six launches).  A
+// workgroup owns a piece of every `step`-th row, reads all ids, and lists the tokens of its rows in order
 // (every wavefront those of a contiguous share).  Then its wavefronts take the rows one by one, and together those of
 // many tokens, each wavefront the tokens of its share.
 constexpr size_t FEW_TOKENS = 2048;
@@ -640,7 +641,7 @@ struct GradPlan {
     size_t at_parts, bytes;
     GradPlan(const size_t n, const size_t rows, const size_t d) : sort(n, rows, false) {
         // The additions of a chunk, and of a row's chunks, are chains: short chunks give more wavefronts and more sums to join
-        // (the whole call for 65,536 tokens of text: chunks of 16 160 us, of 32 168, before loads lost their conditions), longer ones for more tokens keep the joins
+        // (the whole call for 65,536 tokens of text: chunks of 16 160 us, of 32 168), longer ones for more tokens keep the joins
         // short where many are on one row (500,000 tokens on 4 rows: 32 247 us, 64 170, 128 149; a million of text: 32 173, 64
         // 163, 128 185).
         chunk = n <= (size_t(1) << 17) ? 16 : n <= (size_t(1) << 20) ? 64 : 256;
@@ -730,7 +731,7 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
     const auto run = [&](auto sample, auto out_sample) {
         using T = decltype(sample);
         using O = decltype(out_sample);
-        return for_elements<T>(per_lane, [&](auto elements) {
+        return for_elements<std::conditional_t<(sizeof(O) > sizeof(T)), O, T>>(per_lane, [&](auto elements) {
             constexpr int E = decltype(elements)::value;
             GradArgs g{};
             g.grad = d_grad;
