@@ -207,12 +207,13 @@ __device__ __forceinline__ intx4 load16_short(const int8_t* row, const int k, co
 // way: each wavefront requests AHEAD steps of 64 columns before it uses the first.  Bound by memory: 64 matrices of 2,048 x 1,024
 // on 512 rows take 30 us, 4.6 TB/s; one row through 4,096 x 4,096 5.7 us, 3 TB/s, where the launch and one latency are most of it.
 template <class O, int RT, int NB, int WAVES, int AHEAD>
-__global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs p, const uint32_t tiles_n) {
+__global__ __launch_bounds__(WAVES * 64) void product_few_rows_kernel(const ProductArgs p, const uint32_t tiles_n, const uint32_t first_block) {
     constexpr int TM = 16 * RT, TN = 16 * NB;
     __shared__ int part[WAVES][TM][TN + 4];
-    const RowTile rows = find_rows(p, TM, blockIdx.x / tiles_n);
+    const uint32_t block = first_block + blockIdx.x;
+    const RowTile rows = find_rows(p, TM, block / tiles_n);
     if (rows.first >= rows.end) return;
-    const uint32_t n0 = blockIdx.x % tiles_n * TN;
+    const uint32_t n0 = block % tiles_n * TN;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // lane l holds row l % 16 of a block and 16 columns from 16 (l / 16) on
     const int8_t *a[RT], *b[NB];
@@ -329,12 +330,12 @@ struct TileMap {
 };
 
 template <class O, int FM, int FN, int WN>
-__global__ __launch_bounds__(128 * WN, 2) void product_tiles_kernel(const ProductArgs p, const TileMap map) {
+__global__ __launch_bounds__(128 * WN, 2) void product_tiles_kernel(const ProductArgs p, const TileMap map, const uint32_t first_block) {
     constexpr int TM = 64 * FM, TN = 32 * WN * FN, ROWS = 16 * WN, NLA = TM / ROWS, NLB = TN / ROWS;  // ROWS of a load by all threads
     constexpr uint32_t STAGE = (TM + TN) * STAGE_K;
     extern __shared__ __align__(16) int8_t lds[];  // [2][TM + TN][STAGE_K]
     uint32_t tile_m, tile_n;
-    if (!map(blockIdx.x, tile_m, tile_n)) return;
+    if (!map(first_block + blockIdx.x, tile_m, tile_n)) return;
     const RowTile rows = find_rows(p, TM, tile_m);
     if (rows.first >= rows.end) return;
     const uint32_t n0 = tile_n * TN;
@@ -481,9 +482,11 @@ template <class O, int RT, int NB, int WAVES, int AHEAD>
 int launch_few_rows(skm_ctx* ctx, const ProductArgs& p) {
     const uint32_t tiles_n = (p.n + 16 * NB - 1) / (16 * NB);
     const uint64_t blocks = ((uint64_t) (p.m + 16 * RT - 1) / (16 * RT) + (p.offsets ? p.groups : 0)) * tiles_n;
-    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
-    product_few_rows_kernel<O, RT, NB, WAVES, AHEAD><<<(unsigned) blocks, WAVES * 64, 0, ctx->stream>>>(p, tiles_n);
-    return check_hip(hipGetLastError(), "product_few_rows_kernel launch");
+    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: more than 2^31 tiles");
+    return launch_in_parts(blocks, [&](const uint32_t first, const unsigned count) {
+        product_few_rows_kernel<O, RT, NB, WAVES, AHEAD><<<count, WAVES * 64, 0, ctx->stream>>>(p, tiles_n, first);
+        return check_hip(hipGetLastError(), "product_few_rows_kernel launch");
+    });
 }
 
 template <class O, int FM, int FN, int WN>
@@ -496,13 +499,15 @@ int launch_tiles(skm_ctx* ctx, const ProductArgs& p) {
     while (super_n < 8 && super_n < tiles_n) super_n *= 2;
     const uint32_t super_m = 32 / super_n, across = (tiles_n + super_n - 1) / super_n;
     const uint64_t supers = (tiles_m + super_m - 1) / super_m * across, blocks = supers * 32;
-    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: too many tiles for one launch");
+    if (blocks > 0x7fffffffULL) return set_error(SKM_ERR_INVALID, "skm_product_i8: more than 2^31 tiles");
     const TileMap map{super_m, super_n, across, tiles_n, (uint32_t) (supers / 8 * 256)};
     const auto launch = [&](auto kernel) {
         SKM_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int) lds),
                           "hipFuncSetAttribute(MaxDynamicSharedMemorySize)"));
-        kernel<<<(unsigned) blocks, 128 * WN, lds, ctx->stream>>>(p, map);
-        return check_hip(hipGetLastError(), "product_tiles_kernel launch");
+        return launch_in_parts(blocks, [&](const uint32_t first, const unsigned count) {  // parts begin at multiples of 8: dies stay
+            kernel<<<count, 128 * WN, lds, ctx->stream>>>(p, map, first);
+            return check_hip(hipGetLastError(), "product_tiles_kernel launch");
+        });
     };
     return launch(product_tiles_kernel<O, FM, FN, WN>);
 }

@@ -442,13 +442,13 @@ __device__ __forceinline__ void fill_rows(const GradArgs& g, const uint32_t unit
 // One launch for both: the chunks, whose wavefronts wait for memory, under the fill.  Bound by memory: 65,536 tokens of 1,536
 // 16-bit elements into 65,536 rows of fp32, 0.6 GB, in 119 us, 5.1 TB/s.
 template <class T, class O, int E>
-__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_kernel(const GradArgs g, const RowSplit s, const uint32_t chunk_blocks) {
-    const uint32_t wave = threadIdx.x >> 6;
-    if (blockIdx.x < chunk_blocks) {
-        const uint64_t unit = (uint64_t) blockIdx.x * (ROWS_THREADS / 64) + wave;
+__global__ __launch_bounds__(ROWS_THREADS) void lookup_grad_kernel(const GradArgs g, const RowSplit s, const uint32_t chunk_blocks, const uint32_t first_block) {
+    const uint32_t wave = threadIdx.x >> 6, block = first_block + blockIdx.x;
+    if (block < chunk_blocks) {
+        const uint64_t unit = (uint64_t) block * (ROWS_THREADS / 64) + wave;
         if (unit < s.units) grad_of_chunk<T, O, E>(g, s, unit);
     } else {
-        const uint64_t unit = (uint64_t) (blockIdx.x - chunk_blocks) * (ROWS_THREADS / 64) + wave;
+        const uint64_t unit = (uint64_t) (block - chunk_blocks) * (ROWS_THREADS / 64) + wave;
         if (unit * FILL_ROWS < g.rows) fill_rows<O, E>(g, (uint32_t) unit);
     }
 }
@@ -484,22 +484,22 @@ constexpr uint32_t JOIN_ALONE = 16;
 constexpr int JOIN_THREADS = 512;
 
 template <class O, int E>
-__global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const GradArgs g, const uint32_t alone_blocks) {
+__global__ __launch_bounds__(JOIN_THREADS) void lookup_grad_join_kernel(const GradArgs g, const uint32_t alone_blocks, const uint32_t first_block) {
     constexpr int WAVES = JOIN_THREADS / 64;
     __shared__ vec_of<float, E> share[WAVES][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, block = first_block + blockIdx.x;
     const size_t stride = (size_t) 2 * g.d;
     uint32_t c, piece;
     Crossing x;
-    const bool alone = blockIdx.x < alone_blocks;
+    const bool alone = block < alone_blocks;
     if (alone) {
-        const uint64_t unit = (uint64_t) blockIdx.x * WAVES + wave;
+        const uint64_t unit = (uint64_t) block * WAVES + wave;
         if (unit >= (uint64_t) g.chunks * g.pieces) return;
         c = (uint32_t) (unit / g.pieces), piece = (uint32_t) (unit % g.pieces);
         x = crossing_row(g, c);
         if (x.parts == 0 || x.parts > JOIN_ALONE) return;
     } else {
-        const uint32_t unit = blockIdx.x - alone_blocks, c0 = unit / g.pieces * JOIN_ALONE;
+        const uint32_t unit = block - alone_blocks, c0 = unit / g.pieces * JOIN_ALONE;
         piece = unit % g.pieces;
         // lane i < JOIN_ALONE: does a row begin in chunk c0 + i that holds the first token of the JOIN_ALONE chunks after it
         const uint64_t from = (uint64_t) (c0 + lane) * g.chunk, far = from + (uint64_t) JOIN_ALONE * g.chunk;
@@ -545,14 +545,14 @@ template <int E>
 constexpr int FEW_VECTORS = E >= 8 ? 2 : 4;  // vectors a lane holds of a row, at most
 
 template <class T, class O, int E, int V>  // V: vectors a lane holds of a row
-__global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const GradArgs g, const KeySource source, const uint32_t step) {
+__global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const GradArgs g, const KeySource source, const uint32_t step, const uint32_t first_block) {
     constexpr int WAVES = FEW_THREADS / 64, SHARE = FEW_TOKENS / WAVES;
     __shared__ uint32_t listed[WAVES][SHARE];  // number of the row, token
     __shared__ uint32_t many[WAVES], of_row[FEW_ROWS];
     __shared__ vec_of<float, E> share[WAVES][V][64];
     const T* grad = reinterpret_cast<const T*>(g.grad);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t mine = (g.rows - blockIdx.x + step - 1) / step;  // rows blockIdx.x, + step, ...
+    const uint32_t block = first_block + blockIdx.x, mine = (g.rows - 1 - block) / step + 1;  // rows block, + step, ...
     if (threadIdx.x < FEW_ROWS) of_row[threadIdx.x] = 0;
     uint32_t id[SHARE / 64];
 #pragma unroll
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
 #pragma unroll
     for (int q = 0; q < SHARE / 64; ++q) {
         const uint32_t r = id[q] / step;
-        const bool here = id[q] < source.limit && id[q] - r * step == blockIdx.x;
+        const bool here = id[q] < source.limit && id[q] - r * step == block;
         const unsigned long long who = __ballot(here);
         if (here) {
             listed[wave][count + (uint32_t) __popcll(who & lanes_below(lane))] = r << 16 | (wave * SHARE + q * 64 + lane);
@@ -603,7 +603,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
         }
     };
     const auto put = [&](const uint32_t r, const uint32_t at, const vec_of<float, E> (&sum)[V]) {
-        O* out = reinterpret_cast<O*>(g.out) + (size_t) (r * step + blockIdx.x) * g.out_stride;
+        O* out = reinterpret_cast<O*>(g.out) + (size_t) (r * step + block) * g.out_stride;
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (at + i * 64 < g.vectors) put_sum<O, E>(out + column<E>(at + i * 64, g.last), sum[i], g.scale, g.accumulate);
@@ -752,8 +752,10 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
                 const auto launch = [&](auto held) {
                     constexpr int V = decltype(held)::value;
                     const uint32_t pieces = (g.vectors + 64 * V - 1) / (64 * V);
-                    lookup_grad_few_kernel<T, O, E, V><<<dim3(step, pieces), FEW_THREADS, 0, ctx->stream>>>(g, source, step);
-                    return check_hip(hipGetLastError(), "lookup_grad_few_kernel launch");
+                    return launch_in_parts(step, [&](const uint32_t first, const unsigned blocks) {
+                        lookup_grad_few_kernel<T, O, E, V><<<dim3(blocks, pieces), FEW_THREADS, 0, ctx->stream>>>(g, source, step, first);
+                        return check_hip(hipGetLastError(), "lookup_grad_few_kernel launch");
+                    });
                 };
                 if (g.vectors <= 64) return launch(std::integral_constant<int, 1>{});
                 if (g.vectors <= 128) return launch(std::integral_constant<int, 2>{});
@@ -761,29 +763,33 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
                 return launch(std::integral_constant<int, FEW_VECTORS<E>>{});
             }
             const GradPlan plan(n, rows, d);
-            void* at = nullptr;
-            SKM_TRY(call_scratch(ctx, "skm_lookup_rows_grad", d_scratch, scratch_bytes, plan.bytes, &at));
-            char* scratch = (char*) at;
-            SKM_TRY(launch_sort(ctx, plan.sort, source, scratch, nullptr));
-            g.keys = (const uint32_t*) (scratch + plan.sort.at_keys[plan.sort.last()]);
-            g.index = (const uint32_t*) (scratch + plan.sort.at_index[plan.sort.last()]);
             g.chunk = plan.chunk;
             g.chunks = plan.chunks;
-            g.parts = (float*) (scratch + plan.at_parts);
             const RowSplit s = split_rows(plan.chunks, d, E, GRAD_VECTORS);
             constexpr uint64_t PER_BLOCK = ROWS_THREADS / 64;
             const uint64_t chunk_blocks = (s.units + PER_BLOCK - 1) / PER_BLOCK;
             const uint64_t fill_units = accumulate ? 0 : (rows + FILL_ROWS - 1) / FILL_ROWS;
             const uint64_t blocks = chunk_blocks + (fill_units + PER_BLOCK - 1) / PER_BLOCK;
             if (blocks > 0x7fffffffULL || (uint64_t) g.chunks * g.pieces > 0x7fffffffULL)
-                return set_error(SKM_ERR_INVALID, "skm_lookup_rows_grad: too many rows for one launch");
-            lookup_grad_kernel<T, O, E><<<(unsigned) blocks, ROWS_THREADS, 0, ctx->stream>>>(g, s, (uint32_t) chunk_blocks);
-            SKM_TRY(check_hip(hipGetLastError(), "lookup_grad_kernel launch"));
+                return set_error(SKM_ERR_INVALID, "skm_lookup_rows_grad: more than 2^31 workgroups");
+            void* at = nullptr;
+            SKM_TRY(call_scratch(ctx, "skm_lookup_rows_grad", d_scratch, scratch_bytes, plan.bytes, &at));
+            char* scratch = (char*) at;
+            SKM_TRY(launch_sort(ctx, plan.sort, source, scratch, nullptr));
+            g.keys = (const uint32_t*) (scratch + plan.sort.at_keys[plan.sort.last()]);
+            g.index = (const uint32_t*) (scratch + plan.sort.at_index[plan.sort.last()]);
+            g.parts = (float*) (scratch + plan.at_parts);
+            SKM_TRY(launch_in_parts(blocks, [&](const uint32_t first_block, const unsigned count) {
+                lookup_grad_kernel<T, O, E><<<count, ROWS_THREADS, 0, ctx->stream>>>(g, s, (uint32_t) chunk_blocks, first_block);
+                return check_hip(hipGetLastError(), "lookup_grad_kernel launch");
+            }));
             constexpr uint64_t JOINS = JOIN_THREADS / 64;
             const uint32_t alone_blocks = (uint32_t) (((uint64_t) g.chunks * g.pieces + JOINS - 1) / JOINS);
             const uint32_t long_blocks = (g.chunks + JOIN_ALONE - 1) / JOIN_ALONE * g.pieces;
-            lookup_grad_join_kernel<O, E><<<alone_blocks + long_blocks, JOIN_THREADS, 0, ctx->stream>>>(g, alone_blocks);
-            return check_hip(hipGetLastError(), "lookup_grad_join_kernel launch");
+            return launch_in_parts((uint64_t) alone_blocks + long_blocks, [&](const uint32_t first_block, const unsigned count) {
+                lookup_grad_join_kernel<O, E><<<count, JOIN_THREADS, 0, ctx->stream>>>(g, alone_blocks, first_block);
+                return check_hip(hipGetLastError(), "lookup_grad_join_kernel launch");
+            });
         });
     };
     return for_type(type, [&](auto sample) {

@@ -148,10 +148,19 @@ inline RowSplit split_rows(const size_t n, const size_t d, const size_t elements
     return s;
 }
 constexpr int ROWS_THREADS = 256;
-constexpr uint64_t ROWS_MAX_BLOCKS = uint64_t(1) << 22;  // beyond that a wavefront takes several units
+constexpr uint64_t ROWS_MAX_BLOCKS = uint64_t(1) << 22;  // of a launch; beyond that a wavefront takes several units
 inline unsigned row_blocks(const RowSplit& s) {
     const uint64_t per_block = ROWS_THREADS / 64;
     return (unsigned) std::max<uint64_t>(1, std::min(ROWS_MAX_BLOCKS, (s.units + per_block - 1) / per_block));
+}
+
+// A launch has fewer than 2^32 threads in a dimension, so more workgroups than ROWS_MAX_BLOCKS go in several launches: calls
+// launch(number of the first workgroup, workgroups).  Blocks fit in 32 bits.
+template <class F>
+int launch_in_parts(const uint64_t blocks, F&& launch) {
+    for (uint64_t first = 0; first < blocks; first += ROWS_MAX_BLOCKS)
+        SKM_TRY(launch((uint32_t) first, (unsigned) std::min(ROWS_MAX_BLOCKS, blocks - first)));
+    return SKM_OK;
 }
 
 // Calls f with a value of the element type, and with the elements of a vector, that a call asks for.

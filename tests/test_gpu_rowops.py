@@ -942,3 +942,99 @@ def test_refusals_of_the_library(dev, ops, capi):
         assert lib.skm_last_error(), what
     ops.sync()
     assert np.all(x.host() == 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# sizes past one launch
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+class Block:
+    """A contiguous tensor too large to keep on the host, filled with one 32-bit word; parts of it can be read and set."""
+
+    def __init__(self, capi, ctx, shape, kind, word):
+        self.capi, self.ctx, self.shape, self.dtype, self.kind = capi, ctx, shape, kind, kind
+        size = int(np.prod(shape, dtype=np.int64))
+        self.raw_type = np.dtype(RAW.get(kind, kind))
+        self.memory = ctx.empty(size + 4, self.raw_type)
+        capi.check(ctx.lib.skm_fill_u32(ctx.handle, self.memory.ptr, word, self.memory.nbytes // 4))
+
+    def stride(self):
+        steps, step = [], 1
+        for size in reversed(self.shape):
+            steps.insert(0, step)
+            step *= size
+        return tuple(steps)
+
+    def data_ptr(self):
+        return self.memory.ptr
+
+    def part(self, first, count):
+        """`count` elements from the given one on."""
+        out = np.empty(count, self.raw_type)
+        self.capi.check(self.ctx.lib.skm_download(self.ctx.handle, out.ctypes.data, self.memory.offset(first), out.nbytes))
+        return decode(out, self.kind)
+
+    def put(self, first, x):
+        block = np.ascontiguousarray(encode(x, self.kind))
+        self.capi.check(self.ctx.lib.skm_upload(self.ctx.handle, self.memory.offset(first), block.ctypes.data, block.nbytes))
+
+
+@pytest.fixture
+def block(capi, ctx):
+    made = []
+
+    def make(shape, kind, word=0):
+        made.append(Block(capi, ctx, shape, kind, word))
+        return made[-1]
+
+    yield make
+    for b in made:
+        b.memory.free()
+    ctx.lib.skm_device_cache_trim(0)
+
+
+@pytest.mark.parametrize("n", [5, 3000])
+@pytest.mark.parametrize("rows", [2 ** 29 + 195, 2 ** 30 + 100, 2 ** 32 - 2])
+def test_lookup_grad_of_more_rows_than_a_launch_has_threads(dev, block, ops, n, rows):
+    """A launch has fewer than 2^32 threads: 2^24 workgroups of 256, each for 64 rows, or 2^23 of 512."""
+    g = np.random.default_rng(n)
+    places = np.unique(np.concatenate([[0, 1, rows // 2, rows - 2, rows - 1], g.integers(0, rows, 20)]))
+    ids = np.resize(places, n)
+    grad = g.integers(-2, 3, (n, 1))  # sums of up to 600 of them are whole numbers that every type has
+    out = block((rows, 1), "float16", 0x3C003C00)  # ones
+    ops.lookup_grad(dev(grad, "float16"), dev(ids, "int64"), out)
+    window = 1 << 20
+    for at in sorted({0, rows - window, *(int(v) for v in (np.clip(places - window // 2, 0, rows - window)))}):
+        want = np.zeros(window)
+        inside = (ids >= at) & (ids < at + window)
+        np.add.at(want, ids[inside] - at, grad[inside, 0])
+        assert np.array_equal(out.part(at, window), want)
+
+
+def test_product_of_more_rows_than_a_launch_has_threads(dev, block, ops):
+    """Rows too short for the tiles' loads: 2^23 workgroups of 512 threads and one more."""
+    m, n, k = 2 ** 28 + 5, 8, 8
+    g = np.random.default_rng(0)
+    a, a_scales, out = block((m, k), "int8", 0x01010101), block((m,), "float32", 0x3F800000), block((m, n), "bfloat16", 0)
+    b = g.integers(-3, 4, (n, k))
+    windows = [0, m // 2 - 50, 2 ** 27, m - 100]
+    for at in windows:
+        a.put(at * k, np.full((100, k), at % 5 + 1) * (np.arange(100) % 3 - 1)[:, None])
+    ops.product(a, a_scales, dev(b, "int8"), dev(np.ones(n), "float32"), out)
+    for at in windows:
+        rows = a.part(at * k, 100 * k).reshape(100, k)  # as they are now: two of the windows share rows
+        assert np.array_equal(out.part(at * n, 100 * n).reshape(100, n), rows @ b.T)
+    assert np.array_equal(out.part((m // 4) * n, 100 * n).reshape(100, n), np.tile(b.sum(1), (100, 1)))
+
+
+def test_product_of_more_tiles_than_a_launch_has_threads(dev, block, ops):
+    """65,536 groups of nine rows: 17 million tiles of 64 x 64, 256 threads each."""
+    groups, each, n, k = 65536, 9, 14400, 16
+    m = groups * each
+    g = np.random.default_rng(0)
+    a = g.integers(-4, 5, (m, k))
+    b, b_scales, out = block((groups, n, k), "int8", 0x01010101), block((groups, n), "float32", 0x3F800000), block((m, n), "bfloat16", 0)
+    ops.product(dev(a, "int8"), dev(np.ones(m), "float32"), b, b_scales, out, offsets=dev(np.arange(groups + 1) * each, "int32"))
+    for at in (0, m // 3, m // 2 + 7, m - 20):
+        assert np.array_equal(out.part(at * n, 20 * n).reshape(20, n), np.tile(a[at: at + 20].sum(1)[:, None], (1, n)))
