@@ -272,7 +272,8 @@ int skm_householder_q(skm_ctx* ctx, const double* h_a, size_t d, float* h_out_q)
  *   - A value type is SKM_F32, SKM_F16 or SKM_BF16.  Sums are held in fp32 and rounded once, to nearest even.
  *   - Matrices are row-major; a stride is the distance between rows in elements, at least the row length.  Any alignment to
  *     the element's size serves; loads are 16 bytes wide where pointers, strides and row lengths allow.
- *   - Outputs must not overlap inputs.  Elements between the rows of a strided output stay as they are.
+ *   - Outputs and scratch must not overlap inputs or each other (SKM_ERR_INVALID).  Elements between the rows of a strided output
+ *     stay as they are; another matrix of the same stride in bytes may lie there (columns of one buffer), nothing else.
  *   - An index outside the rows it points into stands for no row (SKM_NO_ROW, which skm_knn leaves in empty slots, and
  *     negative 64-bit ids among them): it is never followed.
  *   - Calls allocate nothing, unless they take scratch and are given none: then it comes from the context's workspace,

@@ -571,7 +571,9 @@ int skm_quantize_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t 
     SKM_REQUIRE(d_x && d_q && d_scales, "null pointer");
     const size_t size = type_size(type);
     SKM_REQUIRE(address(d_x) % size == 0 && address(d_scales) % 4 == 0, "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_x, span(n, x_stride, d, size), d_q, span(n, q_stride, d, 1)), "q overlaps x");
+    const Argument x{"x", matrix_memory(d_x, n, x_stride, d, size)}, q{"q", matrix_memory(d_q, n, q_stride, d, 1)};
+    SKM_TRY(check_apart(__func__, q, {x}));
+    SKM_TRY(check_apart(__func__, {"scales", vector_memory(d_scales, n, 4)}, {x, q}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/quantize");
     return for_type(type, [&](auto sample) {
@@ -602,6 +604,7 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
     SKM_REQUIRE(k > 0 && k <= SKM_PRODUCT_MAX_K, "k out of range");
     SKM_REQUIRE(m <= SKM_PRODUCT_MAX_M, "m out of range");
     SKM_REQUIRE(a_stride >= k && b_stride >= k && out_stride >= n, "strides must be at least the row length");
+    SKM_REQUIRE(b_stride < (size_t(1) << 40) && (!d_offsets || b_group_stride < (size_t(1) << 46)), "strides out of range");
     if (d_offsets) {
         SKM_REQUIRE(groups > 0 && groups <= SKM_PRODUCT_MAX_GROUPS, "groups out of range");
         SKM_REQUIRE(groups == 1 || b_group_stride >= (n - 1) * b_stride + k, "b_group_stride must be at least a group's matrix");
@@ -611,11 +614,15 @@ int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, c
     const size_t out_size = type_size(out_type);
     SKM_REQUIRE((address(d_a_scale) | address(d_b_scale) | address(d_bias) | address(d_offsets)) % 4 == 0 && address(d_out) % out_size == 0,
                 "pointers must be aligned to their elements");
-    const size_t out_bytes = span(m, out_stride, n, out_size);
-    SKM_REQUIRE(!overlap(d_a, span(m, a_stride, k, 1), d_out, out_bytes), "out overlaps a");
-    SKM_REQUIRE(!overlap(d_a_scale, m * 4, d_out, out_bytes) && !overlap(d_b_scale, (d_offsets ? groups : 1) * n * 4, d_out, out_bytes),
-                "out overlaps the scales");
-    SKM_REQUIRE(!overlap(d_b, (d_offsets ? (groups - 1) * b_group_stride : 0) + span(n, b_stride, k, 1), d_out, out_bytes), "out overlaps b");
+    const size_t matrices = d_offsets ? groups : 1;
+    // of several matrices the whole range
+    const Memory b = matrices == 1 ? matrix_memory(d_b, n, b_stride, k, 1)
+                                   : matrix_memory(d_b, 1, (matrices - 1) * b_group_stride + (n - 1) * b_stride + k,
+                                                   (matrices - 1) * b_group_stride + (n - 1) * b_stride + k, 1);
+    SKM_TRY(check_apart(__func__, {"out", matrix_memory(d_out, m, out_stride, n, out_size)},
+                        {{"a", matrix_memory(d_a, m, a_stride, k, 1)}, {"a_scale", vector_memory(d_a_scale, m, 4)}, {"b", b},
+                         {"b_scale", vector_memory(d_b_scale, matrices * n, 4)}, {"the bias", vector_memory(d_bias, matrices * n, 4)},
+                         {"the offsets", vector_memory(d_offsets, d_offsets ? groups + 1 : 0, 4)}}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/product");
     const ProductArgs p{d_a, d_a_scale, d_b, d_b_scale, d_bias, d_offsets, d_out, a_stride, b_stride, d_offsets ? b_group_stride : 0,

@@ -274,8 +274,9 @@ int skm_lookup_rows(skm_ctx* ctx, const void* d_table, int type, size_t rows, si
     const size_t size = type_size(type);
     SKM_REQUIRE(address(d_ids) % (ids_type == SKM_I64 ? 8 : 4) == 0 && address(d_table) % size == 0 && address(d_out) % size == 0,
                 "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_table, span(rows, table_stride, d, size), d_out, span(n, out_stride, d, size)) &&
-                !overlap(d_ids, n * (ids_type == SKM_I64 ? 8 : 4), d_out, span(n, out_stride, d, size)), "out overlaps the table or the ids");
+    SKM_TRY(check_apart(__func__, {"out", matrix_memory(d_out, n, out_stride, d, size)},
+                        {{"the table", matrix_memory(d_table, rows, table_stride, d, size)},
+                         {"the ids", vector_memory(d_ids, n, ids_type == SKM_I64 ? 8 : 4)}}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup");
     return for_type(type, [&](auto sample) {
@@ -309,7 +310,8 @@ int skm_dispatch_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t 
     const size_t size = type_size(type);
     SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_x) % size == 0 && address(d_out) % size == 0,
                 "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_x, span(n, x_stride, d, size), d_out, span(out_rows, out_stride, d, size)), "out overlaps x");
+    SKM_TRY(check_apart(__func__, {"out", matrix_memory(d_out, out_rows, out_stride, d, size)},
+                        {{"x", matrix_memory(d_x, n, x_stride, d, size)}, {"the slots", vector_memory(d_slots, n * choices, 4)}}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/dispatch");
     return for_type(type, [&](auto sample) {
@@ -339,7 +341,9 @@ int skm_combine_rows(skm_ctx* ctx, const void* d_rows, int type, size_t n_rows, 
     const size_t size = type_size(type);
     SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_rows) % size == 0 && address(d_out) % size == 0 &&
                 (!d_weights || address(d_weights) % type_size(weights_type) == 0), "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_rows, span(n_rows, rows_stride, d, size), d_out, span(n, out_stride, d, size)), "out overlaps the rows");
+    SKM_TRY(check_apart(__func__, {"out", matrix_memory(d_out, n, out_stride, d, size)},
+                        {{"the rows", matrix_memory(d_rows, n_rows, rows_stride, d, size)}, {"the slots", vector_memory(d_slots, n * choices, 4)},
+                         {"the weights", vector_memory(d_weights, n * choices, type_size(weights_type))}}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/combine");
     return for_type(type, [&](auto sample) {
@@ -373,12 +377,13 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
     SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_grad) % size == 0 && address(d_rows) % size == 0 &&
                 address(d_grad_rows) % size == 0 && (!d_weights || address(d_weights) % weight_size == 0) &&
                 (!d_grad_weights || address(d_grad_weights) % weight_size == 0), "pointers must be aligned to their elements");
-    if (d_grad_rows) {
-        const size_t bytes = span(n_rows, grad_rows_stride, d, size);
-        SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps grad");
-        SKM_REQUIRE(!d_grad_weights || !overlap(d_rows, span(n_rows, rows_stride, d, size), d_grad_rows, bytes), "grad_rows overlaps the rows");
-    }
-    SKM_REQUIRE(!overlap(d_weights, n * choices * weight_size, d_grad_weights, n * choices * weight_size), "grad_weights overlaps the weights");
+    const Argument grad_rows{"grad_rows", matrix_memory(d_grad_rows, d_grad_rows ? n_rows : 0, grad_rows_stride, d, size)};
+    const Argument grad_weights{"grad_weights", vector_memory(d_grad_weights, n * choices, weight_size)};
+    const Argument grad{"grad", matrix_memory(d_grad, n, grad_stride, d, size)}, slots{"the slots", vector_memory(d_slots, n * choices, 4)};
+    const Argument weights{"the weights", vector_memory(d_weights, n * choices, weight_size)};
+    const Argument rows{"the rows", matrix_memory(d_rows, d_grad_weights ? n_rows : 0, rows_stride, d, size)};  // else not read
+    SKM_TRY(check_apart(__func__, grad_rows, {grad, slots, weights, rows, grad_weights}));
+    SKM_TRY(check_apart(__func__, grad_weights, {grad, slots, weights, rows}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/combine_grad");
     return for_type(type, [&](auto sample) {

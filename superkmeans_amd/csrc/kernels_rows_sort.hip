@@ -677,10 +677,12 @@ int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices,
     SKM_REQUIRE((address(d_choices) | address(d_slots) | address(d_order) | address(d_offsets)) % 4 == 0,
                 "pointers must be aligned to their elements");
     const size_t places = n * choices;
-    SKM_REQUIRE(!overlap(d_choices, places * 4, d_slots, places * 4) && !overlap(d_choices, places * 4, d_order, places * 4) &&
-                !overlap(d_slots, places * 4, d_order, places * 4) && !overlap(d_slots, places * 4, d_offsets, (groups + 1) * 4) &&
-                !overlap(d_choices, places * 4, d_offsets, (groups + 1) * 4) && !overlap(d_order, places * 4, d_offsets, (groups + 1) * 4),
-                "choices, slots, order and offsets must not overlap");
+    const Argument from{"the choices", vector_memory(d_choices, places, 4)}, slots{"slots", vector_memory(d_slots, places, 4)};
+    const Argument order{"order", vector_memory(d_order, places, 4)}, offsets{"offsets", vector_memory(d_offsets, groups + 1, 4)};
+    SKM_TRY(check_apart(__func__, slots, {from, order, offsets}));
+    SKM_TRY(check_apart(__func__, order, {from, offsets}));
+    SKM_TRY(check_apart(__func__, offsets, {from}));
+    SKM_TRY(check_apart(__func__, {"scratch", vector_memory(d_scratch, need, 1)}, {from, slots, order, offsets}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/route");
     if (places == 0) return skm_fill_u32(ctx, d_offsets, 0, groups + 1);
@@ -688,8 +690,8 @@ int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices,
     void* scratch = nullptr;
     SKM_TRY(call_scratch(ctx, __func__, d_scratch, scratch_bytes, plan.bytes, &scratch));
     const KeySource source{d_choices, SKM_U32, (uint32_t) groups};
-    const Places out{nullptr, nullptr, nullptr, d_slots, d_order, d_offsets};
-    if (plan.passes == 1) return launch_sort(ctx, plan, source, (char*) scratch, &out);
+    const Places places_out{nullptr, nullptr, nullptr, d_slots, d_order, d_offsets};
+    if (plan.passes == 1) return launch_sort(ctx, plan, source, (char*) scratch, &places_out);
     SKM_TRY(launch_sort(ctx, plan, source, (char*) scratch, nullptr));
     const uint32_t* keys = (const uint32_t*) ((char*) scratch + plan.at_keys[plan.last()]);
     const uint32_t* index = (const uint32_t*) ((char*) scratch + plan.at_index[plan.last()]);
@@ -722,7 +724,11 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
     const size_t size = type_size(type), out_size = type_size(out_type);
     SKM_REQUIRE(address(d_ids) % (ids_type == SKM_I64 ? 8 : 4) == 0 && address(d_grad) % size == 0 && address(d_out) % out_size == 0,
                 "pointers must be aligned to their elements");
-    SKM_REQUIRE(!overlap(d_grad, span(n, grad_stride, d, size), d_out, span(rows, out_stride, d, out_size)), "out overlaps the gradient");
+    const Argument grad{"grad", matrix_memory(d_grad, n, grad_stride, d, size)};
+    const Argument ids{"the ids", vector_memory(d_ids, n, ids_type == SKM_I64 ? 8 : 4)};
+    const Argument out{"out", matrix_memory(d_out, rows, out_stride, d, out_size)};
+    SKM_TRY(check_apart(__func__, out, {grad, ids}));
+    SKM_TRY(check_apart(__func__, {"scratch", vector_memory(d_scratch, need, 1)}, {grad, ids, out}));
     OnDevice on(ctx);
     ScopedStage st(ctx, "rows/lookup_grad");
     // an accumulated vector must not be added twice

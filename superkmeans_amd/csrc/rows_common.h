@@ -5,6 +5,7 @@
 #include "skm_internal.h"
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace skm {
@@ -80,12 +81,41 @@ inline bool is_value_type(const int type) { return type == SKM_F32 || type == SK
 
 inline size_t address(const void* p) { return reinterpret_cast<size_t>(p); }
 
-inline bool overlap(const void* a, const size_t a_bytes, const void* b, const size_t b_bytes) {
-    return a && b && address(a) < address(b) + b_bytes && address(b) < address(a) + a_bytes;
+// The memory of an argument: `rows` pieces of `width` bytes, `pitch` bytes from one to the next (no less than the width).
+struct Memory {
+    size_t at, rows, pitch, width;
+    size_t length() const { return rows ? (rows - 1) * pitch + width : 0; }
+};
+inline Memory matrix_memory(const void* p, const size_t rows, const size_t stride, const size_t d, const size_t size) {
+    if (!p || rows == 0) return {0, 0, 0, 0};
+    size_t last;
+    // a distance that no address space has: all of it
+    if (__builtin_mul_overflow(stride, size, &last) || __builtin_mul_overflow(rows, last, &last) || last > SIZE_MAX - address(p))
+        return {0, 1, SIZE_MAX, SIZE_MAX};
+    if (stride == d) return {address(p), 1, rows * d * size, rows * d * size};
+    return {address(p), rows, stride * size, d * size};
 }
-// Bytes from the first to the last element of a matrix.
-inline size_t span(const size_t rows, const size_t stride, const size_t d, const size_t size) {
-    return rows ? ((rows - 1) * stride + d) * size : 0;
+inline Memory vector_memory(const void* p, const size_t n, const size_t size) { return matrix_memory(p, n, 1, 1, size); }
+
+// Whether the ranges of two arguments meet, from the first byte to the last: where both have rows of one pitch, as views of
+// columns of one buffer do, whether their rows meet.
+inline bool meet(const Memory& a, const Memory& b) {
+    if (a.rows == 0 || b.rows == 0) return false;
+    if (a.at >= b.at + b.length() || b.at >= a.at + a.length()) return false;
+    if (a.pitch != b.pitch) return true;
+    const size_t past = b.at >= a.at ? (b.at - a.at) % a.pitch : (a.pitch - (a.at - b.at) % a.pitch) % a.pitch;
+    return past < a.width || past + b.width > a.pitch;
+}
+
+struct Argument {
+    const char* name;
+    Memory memory;
+};
+// SKM_ERR_INVALID where an output shares memory with an argument that is read, or with another output.
+inline int check_apart(const char* who, const Argument& out, const std::initializer_list<Argument> others) {
+    for (const Argument& other : others)
+        if (meet(out.memory, other.memory)) return set_error(SKM_ERR_INVALID, "%s: %s overlaps %s", who, out.name, other.name);
+    return SKM_OK;
 }
 
 // The calling thread's device is the context's while an entry point launches, and what it was afterwards (the default

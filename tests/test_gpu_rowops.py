@@ -1038,3 +1038,55 @@ def test_product_of_more_tiles_than_a_launch_has_threads(dev, block, ops):
     ops.product(dev(a, "int8"), dev(np.ones(m), "float32"), b, b_scales, out, offsets=dev(np.arange(groups + 1) * each, "int32"))
     for at in (0, m // 3, m // 2 + 7, m - 20):
         assert np.array_equal(out.part(at * n, 20 * n).reshape(20, n), np.tile(a[at: at + 20].sum(1)[:, None], (1, n)))
+
+
+class Columns:
+    """Some columns of a tensor in device memory."""
+
+    def __init__(self, whole, first, count):
+        self.whole, self.first, self.count = whole, first, count
+        self.shape, self.dtype, self.kind = (whole.shape[0], count), whole.dtype, whole.kind
+
+    def stride(self):
+        return self.whole.stride()
+
+    def data_ptr(self):
+        return self.whole.memory.offset(self.first)
+
+    def host(self):
+        return self.whole.host()[:, self.first: self.first + self.count]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [1, 7, 64, 515])
+def test_inputs_and_outputs_in_columns_of_one_buffer(dev, ops, kind, d):
+    """Results between the rows of their inputs: nothing else of the buffer changes."""
+    g = np.random.default_rng(d)
+    n, k = 60, 3
+    start = typed(g.standard_normal((n * k, 3 * d + 5)), kind)
+    whole = dev(start, kind)
+    left, middle, right = (Columns(whole, at, d) for at in (1, d + 2, 2 * d + 3))
+    want = start.copy()
+
+    def check(columns, values):
+        want[:, columns.first: columns.first + d] = values
+        assert np.array_equal(whole.host(), want)
+
+    ids = g.integers(0, n * k, n * k)
+    ops.lookup(left, dev(ids, "int32"), middle)
+    check(middle, start[ids, 1: 1 + d])
+    slots = g.permutation(n * k).reshape(n * k, 1)
+    ops.dispatch(middle, dev(slots, "int32"), right)
+    there = np.empty((n * k, d))
+    there[slots[:, 0]] = middle.host()
+    check(right, there)
+    ops.combine(right, dev(slots, "int32"), left)
+    check(left, there[slots[:, 0]])
+    ops.combine_grad(left, right, dev(slots, "int32"), None, middle, None)
+    scattered = np.empty((n * k, d))
+    scattered[slots[:, 0]] = left.host()
+    check(middle, scattered)
+    ops.lookup_grad(middle, dev(slots[:, 0], "int64"), right)
+    again = np.empty((n * k, d))
+    again[slots[:, 0]] = scattered
+    check(right, again)

@@ -166,3 +166,106 @@ def test_null_context_is_refused(capi):
     assert lib.skm_route(None, None, 1, 1, 1, None, None, None, None, 0) == capi.SKM_ERR_INVALID
     assert lib.skm_product_i8(None, None, 1, 1, None, None, 1, 1, 1, None, None, 0, 0, None, None, 0, 1) == capi.SKM_ERR_INVALID
     assert lib.skm_quantize_rows(None, None, 0, 1, 1, 1, None, 1, None) == capi.SKM_ERR_INVALID
+
+
+# Every entry with its arguments apart: name -> (rows, pitch, width) in bytes, and the call for a set of addresses (of the scratch the
+# first bytes, all of which the calls need).
+N, D, K, ROWS = 6, 8, 3, 9
+ENTRIES = {
+    "skm_lookup_rows": (
+        {"table": (ROWS, 40, 32), "ids": (1, 48, 48), "out": (N, 48, 32)}, {"out": ("table", "ids")},
+        lambda f, h, a: f(h, a["table"], 0, ROWS, D, 10, a["ids"], 4, N, 1.0, a["out"], 12)),
+    "skm_lookup_rows_grad": (
+        {"grad": (3000, 40, 32), "ids": (1, 24000, 24000), "out": (ROWS, 48, 32), "scratch": (1, 4096, 4096)},
+        {"out": ("grad", "ids", "scratch"), "scratch": ("grad", "ids")},
+        lambda f, h, a: f(h, a["grad"], 0, 10, a["ids"], 4, 3000, ROWS, D, 1.0, a["out"], 0, 12, 0, a["scratch"], 1 << 20)),
+    "skm_route": (
+        {"choices": (1, 120000, 120000), "slots": (1, 120000, 120000), "order": (1, 120000, 120000), "offsets": (1, 20, 20), "scratch": (1, 4096, 4096)},
+        {"slots": ("choices", "order", "offsets"), "order": ("choices", "offsets"), "offsets": ("choices",),
+         "scratch": ("choices", "slots", "order", "offsets")},
+        lambda f, h, a: f(h, a["choices"], 10000, 3, 4, a["slots"], a["order"], a["offsets"], a["scratch"], 1 << 20)),
+    "skm_dispatch_rows": (
+        {"x": (N, 40, 32), "slots": (1, 72, 72), "out": (18, 48, 32)}, {"out": ("x", "slots")},
+        lambda f, h, a: f(h, a["x"], 0, N, D, 10, a["slots"], K, a["out"], 18, 12)),
+    "skm_combine_rows": (
+        {"rows": (18, 40, 32), "slots": (1, 72, 72), "weights": (1, 36, 36), "out": (N, 48, 32)}, {"out": ("rows", "slots", "weights")},
+        lambda f, h, a: f(h, a["rows"], 0, 18, D, 10, a["slots"], N, K, a["weights"], 1, a["out"], 12)),
+    "skm_combine_rows_grad": (
+        {"grad": (N, 40, 32), "rows": (18, 40, 32), "slots": (1, 72, 72), "weights": (1, 72, 72), "grad_rows": (18, 48, 32),
+         "grad_weights": (1, 72, 72)},
+        {"grad_rows": ("grad", "rows", "slots", "weights", "grad_weights"), "grad_weights": ("grad", "rows", "slots", "weights")},
+        lambda f, h, a: f(h, a["grad"], 0, N, D, 10, a["rows"], 18, 10, a["slots"], K, a["weights"], 0, a["grad_rows"], 12, a["grad_weights"])),
+    "skm_quantize_rows": (
+        {"x": (N, 40, 32), "q": (N, 12, 8), "scales": (1, 24, 24)}, {"q": ("x",), "scales": ("x", "q")},
+        lambda f, h, a: f(h, a["x"], 0, N, D, 10, a["q"], 12, a["scales"])),
+    "skm_product_i8": (
+        {"a": (N, 12, 8), "a_scale": (1, 24, 24), "b": (1, 120, 120), "b_scale": (1, 40, 40), "bias": (1, 40, 40), "offsets": (1, 12, 12),
+         "out": (N, 32, 20)},
+        {"out": ("a", "a_scale", "b", "b_scale", "bias", "offsets")},
+        lambda f, h, a: f(h, a["a"], N, 12, a["a_scale"], a["b"], 5, D, 12, a["b_scale"], a["bias"], 2, 60, a["offsets"], a["out"], 0, 8)),
+}
+PAIRS = [(entry, out, other) for entry, (_, pairs, _) in ENTRIES.items() for out, others in pairs.items() for other in others]
+
+
+@pytest.fixture
+def refusing(capi):
+    """The library with memory that is no context: a call that is refused never looks at it, one that is not finds no device."""
+    import ctypes
+
+    lib = capi.load()
+    if capi.device_count() > 0:
+        pytest.skip("the addresses here are no memory: without a device only")
+    memory = ctypes.create_string_buffer(1 << 16)
+    return lib, ctypes.addressof(memory), memory
+
+
+def apart(entry):
+    return {name: (i + 1) << 32 for i, name in enumerate(ENTRIES[entry][0])}
+
+
+@pytest.mark.parametrize("entry", sorted(ENTRIES))
+def test_arguments_that_are_apart_are_not_refused(refusing, capi, entry):
+    lib, handle, _ = refusing
+    assert ENTRIES[entry][2](getattr(lib, entry), handle, apart(entry)) not in (0, capi.SKM_ERR_INVALID)
+
+
+@pytest.mark.parametrize("entry,out,other", PAIRS)
+def test_outputs_over_other_arguments_are_refused(refusing, capi, entry, out, other):
+    lib, handle, _ = refusing
+    shapes, _, call = ENTRIES[entry]
+    at = apart(entry)
+    (rows, pitch, width), (other_rows, other_pitch, other_width) = shapes[out], shapes[other]
+    end = (other_rows - 1) * other_pitch + other_width
+    for place in (at[other], at[other] + (end - 1) // 16 * 16):  # the same beginning, and the other's last bytes
+        if rows == 1 and other_rows > 1 and place != at[other]:
+            place = at[other] + (other_rows - 1) * other_pitch // 16 * 16
+        assert call(getattr(lib, entry), handle, {**at, out: place}) == capi.SKM_ERR_INVALID, (entry, out, other)
+        message = lib.skm_last_error().decode()
+        assert "overlaps" in message and entry in message, message
+
+
+def test_columns_of_one_buffer_are_apart(refusing, capi):
+    """Rows that lie between each other's rows share no memory; one byte more and they do."""
+    lib, handle, _ = refusing
+    at = 1 << 32
+
+    def dispatch(x, out, x_stride, out_stride, d, slots=1 << 40):
+        return lib.skm_dispatch_rows(handle, x, 0, 50, d, x_stride, slots, 1, out, 50, out_stride)
+
+    assert dispatch(at, at + 32, 16, 16, 8) != capi.SKM_ERR_INVALID
+    assert dispatch(at + 32, at, 16, 16, 8) != capi.SKM_ERR_INVALID
+    assert dispatch(at + 160, at, 16, 16, 8) != capi.SKM_ERR_INVALID  # 2.5 rows on
+    assert dispatch(at, at + 32, 16, 16, 9) == capi.SKM_ERR_INVALID
+    assert dispatch(at, at + 28, 16, 16, 8) == capi.SKM_ERR_INVALID
+    assert dispatch(at, at + 32, 16, 17, 8) == capi.SKM_ERR_INVALID  # other pitches: their rows meet somewhere
+    # vectors are apart from the whole range of a result's rows
+    assert dispatch(1 << 33, at, 256, 256, 8, slots=at + 32) == capi.SKM_ERR_INVALID
+    assert dispatch(1 << 33, at, 256, 256, 8, slots=at - 200) != capi.SKM_ERR_INVALID
+    assert dispatch(1 << 33, at, 256, 256, 8, slots=at - 196) == capi.SKM_ERR_INVALID
+    assert dispatch(1 << 33, at, 256, 256, 8, slots=at + 1024 * 49 + 32) != capi.SKM_ERR_INVALID
+    # a single row between the rows of the result
+    assert lib.skm_dispatch_rows(handle, at, 0, 1, 8, 16, 1 << 40, 1, at + 32, 50, 16) != capi.SKM_ERR_INVALID
+    assert lib.skm_dispatch_rows(handle, at + 64 * 7, 0, 1, 8, 16, 1 << 40, 1, at + 32, 50, 16) != capi.SKM_ERR_INVALID
+    assert lib.skm_dispatch_rows(handle, at + 64 * 7 + 4, 0, 1, 8, 16, 1 << 40, 1, at + 32, 50, 16) == capi.SKM_ERR_INVALID
+    # distances that wrap
+    assert dispatch(1 << 33, at, 16, 1 << 60, 8) == capi.SKM_ERR_INVALID
