@@ -55,6 +55,7 @@ int skm_ctx_create(int device, skm_ctx** out_ctx);
  * memory).  The calling thread's current device is left as it was.  No counterpart in the reference. */
 int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx);
 int skm_ctx_destroy(skm_ctx* ctx);
+int skm_ctx_get_device(const skm_ctx* ctx, int* out_device);
 int skm_sync(skm_ctx* ctx);
 /* Upper bound, in bytes, of the scratch a single stage call may allocate (default 24 GiB of the
  * 288 GB of HBM: large enough that the headline shapes run as one launch per stage). */

@@ -25,6 +25,7 @@ _PROTOTYPES = {
     "skm_ctx_create": (c_int, [c_int, POINTER(c_void_p)]),
     "skm_ctx_create_on_stream": (c_int, [c_int, c_void_p, POINTER(c_void_p)]),
     "skm_ctx_destroy": (c_int, [c_void_p]),
+    "skm_ctx_get_device": (c_int, [c_void_p, POINTER(c_int)]),
     "skm_sync": (c_int, [c_void_p]),
     "skm_ctx_set_workspace_limit": (c_int, [c_void_p, c_size_t]),
     "skm_ctx_set_candidate_kernel": (c_int, [c_void_p, c_int]),
@@ -242,6 +243,10 @@ class DeviceArray:
     def data_ptr(self):
         return self.ptr
 
+    def get_device(self):
+        """Number of the device that the memory is on."""
+        return self.ctx.device
+
     def offset(self, elements):
         """Device address `elements` items past the start."""
         return self.ptr + int(elements) * self.dtype.itemsize
@@ -254,6 +259,12 @@ class DeviceArray:
                 self.ctx._live.remove(self)
             except ValueError:
                 pass
+
+
+def _device_of(lib, handle):
+    device = c_int()
+    check(lib.skm_ctx_get_device(handle, ctypes.byref(device)))
+    return device.value
 
 
 class Context:
@@ -272,6 +283,7 @@ class Context:
         else:
             check(self.lib.skm_ctx_create_on_stream(device, c_void_p(stream), ctypes.byref(h)))
         self.handle = h.value
+        self.device = _device_of(self.lib, self.handle)
         self._live = []
 
     def close(self):
@@ -325,6 +337,7 @@ class _BorrowedContext(Context):
     def __init__(self, handle):
         self.lib = load()
         self.handle = handle
+        self.device = _device_of(self.lib, handle)
         self._live = []
 
     def close(self):

@@ -326,6 +326,13 @@ int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx) {
     return create_context(device, false, stream, out_ctx);
 }
 
+int skm_ctx_get_device(const skm_ctx* ctx, int* out_device) {
+    SKM_REQUIRE(ctx, "null context");
+    SKM_REQUIRE(out_device, "null output");
+    *out_device = ctx->device;
+    return SKM_OK;
+}
+
 int skm_ctx_destroy(skm_ctx* ctx) {
     if (!ctx) return SKM_OK;
     const DeviceAsItWas as_it_was(!ctx->owns_stream);

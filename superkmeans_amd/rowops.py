@@ -61,8 +61,8 @@ class RowOperators:
 
     Parameters
     ----------
-    device : int
-        Device of every tensor that the calls get.
+    device : int or None
+        Device of every tensor that the calls get: 0, or the context's where one is given.
     stream : int or None
         Handle of the stream to queue on (0: the device's default stream); it has to outlive the object.  None: a stream of
         the object's own, which callers order with their work through ``sync``.
@@ -72,10 +72,18 @@ class RowOperators:
     An object is not thread-safe: calls from several threads take an object each.
     """
 
-    def __init__(self, device=0, stream=None, ctx=None):
+    def __init__(self, device=None, stream=None, ctx=None):
+        self.ctx = None
         self._owned = ctx is None
-        self.ctx = _capi.Context(device, stream) if ctx is None else ctx
-        self.device = device
+        if ctx is not None:
+            has = getattr(ctx, "device", device)
+            if device not in (None, has):
+                raise ValueError(f"the context is on device {has}, not on device {device}")
+            if stream is not None:
+                raise ValueError("a context has its stream already")
+            device = has
+        self.device = 0 if device is None else device
+        self.ctx = _capi.Context(self.device, stream) if ctx is None else ctx
         self._lib = self.ctx.lib
         self._handle = self.ctx.handle
 
@@ -112,7 +120,7 @@ class RowOperators:
             where = getattr(x, "device", None)
             index = self.device if where is None else where.index if getattr(where, "type", "cuda") == "cuda" else -1
         if index != self.device:
-            raise ValueError(f"{what} is on {x.device}, not on device {self.device}")
+            raise ValueError(f"{what} is on {getattr(x, 'device', f'device {index}')}, not on device {self.device}")
         return x.data_ptr() or None
 
     def _refuse(self, x, what, error):

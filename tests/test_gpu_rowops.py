@@ -1090,3 +1090,13 @@ def test_inputs_and_outputs_in_columns_of_one_buffer(dev, ops, kind, d):
     again = np.empty((n * k, d))
     again[slots[:, 0]] = scattered
     check(right, again)
+
+
+def test_arrays_know_their_device(capi, ctx, ops):
+    assert ctx.device == ops.device == 0
+    a = ctx.array(np.ones((2, 4), np.float32))
+    assert a.get_device() == 0
+    km = capi.KMeans(4, 8)
+    assert km.ctx.device == 0
+    km.close()
+    a.free()

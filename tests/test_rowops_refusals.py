@@ -269,3 +269,48 @@ def test_columns_of_one_buffer_are_apart(refusing, capi):
     assert lib.skm_dispatch_rows(handle, at + 64 * 7 + 4, 0, 1, 8, 16, 1 << 40, 1, at + 32, 50, 16) == capi.SKM_ERR_INVALID
     # distances that wrap
     assert dispatch(1 << 33, at, 16, 1 << 60, 8) == capi.SKM_ERR_INVALID
+
+
+class ContextOfDevice(Context):
+    def __init__(self, device):
+        super().__init__()
+        self.device = device
+
+
+class Owned(Tensor):
+    """An allocation that knows its context, and through it the device."""
+
+    def __init__(self, ctx, *args, **kw):
+        super().__init__(*args, **kw)
+        self.ctx = ctx
+        del self.device
+
+    def get_device(self):
+        return self.ctx.device
+
+
+def test_tensors_are_compared_with_the_context_s_device():
+    ctx, elsewhere = ContextOfDevice(1), ContextOfDevice(0)
+    there, here = Device("cuda", 1), Device("cuda", 0)
+    with rowops.RowOperators(ctx=ctx) as ops:
+        assert ops.device == 1
+        ops.lookup(T((9, 4), device=there), I((3,), device=there), T((3, 4), device=there))
+        ops.lookup(Owned(ctx, (9, 4)), Owned(ctx, (3,), "int32"), Owned(ctx, (3, 4)))
+        assert len(ctx.lib.calls) == 2
+        for bad in (lambda: ops.lookup(T((9, 4), device=here), I((3,), device=there), T((3, 4), device=there)),
+                    lambda: ops.lookup(Owned(elsewhere, (9, 4)), Owned(ctx, (3,), "int32"), Owned(ctx, (3, 4)))):
+            with pytest.raises(ValueError, match="not on device 1"):
+                bad()
+        assert len(ctx.lib.calls) == 2
+    with pytest.raises(ValueError, match="device 1, not on device 0"):
+        rowops.RowOperators(device=0, ctx=ctx)
+    with pytest.raises(ValueError, match="stream"):
+        rowops.RowOperators(stream=7, ctx=ctx)
+    assert rowops.RowOperators(device=1, ctx=ctx).device == 1
+
+
+def test_device_of_no_context(capi):
+    import ctypes
+
+    device = ctypes.c_int(7)
+    assert capi.load().skm_ctx_get_device(None, ctypes.byref(device)) == capi.SKM_ERR_INVALID
