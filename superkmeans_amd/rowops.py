@@ -67,7 +67,7 @@ class RowOperators:
         Handle of the stream to queue on (0: the device's default stream); it has to outlive the object.  None: a stream of
         the object's own, which callers order with their work through ``sync``.
     ctx : Context or None
-        An existing context to work on instead.
+        An existing context to work on instead; the object is of no use once that is closed.
 
     An object is not thread-safe: calls from several threads take an object each.
     """
@@ -85,13 +85,17 @@ class RowOperators:
         self.device = 0 if device is None else device
         self.ctx = _capi.Context(self.device, stream) if ctx is None else ctx
         self._lib = self.ctx.lib
-        self._handle = self.ctx.handle
+
+    @property
+    def _handle(self):
+        """None once the object or the context is closed: the library refuses a null context."""
+        return self.ctx.handle if self.ctx is not None else None
 
     def close(self):
         """Releases the context, if it is the object's own."""
         if self._owned and self.ctx is not None:
             self.ctx.close()
-        self.ctx = self._handle = None  # a call after this is refused by the library: null context
+        self.ctx = None
 
     def __enter__(self):
         return self
@@ -107,7 +111,7 @@ class RowOperators:
 
     def sync(self):
         """Waits for the stream."""
-        self.ctx.sync()
+        self._call(self._lib.skm_sync(self._handle))
 
     # -- arguments ---------------------------------------------------------------------------------------------------
     # A decoding step's calls are short: these checks are written for few attribute reads, not for few lines.

@@ -314,3 +314,21 @@ def test_device_of_no_context(capi):
 
     device = ctypes.c_int(7)
     assert capi.load().skm_ctx_get_device(None, ctypes.byref(device)) == capi.SKM_ERR_INVALID
+
+
+def test_a_closed_context_is_not_used_again(capi):
+    """The handle of a context is taken for each call: a closed one has none, and the library refuses that."""
+    ctx = Context()
+    ops = rowops.RowOperators(ctx=ctx)
+    ctx.handle = None  # what Context.close leaves
+    ops.lookup(T((9, 4)), I((3,)), T((3, 4)))
+    ops.sync()
+    assert [args[0] for _, args in ctx.lib.calls] == [None, None]
+    ctx.lib, ctx.handle = capi.load(), None
+    for closed in (False, True):
+        ops = rowops.RowOperators(ctx=ctx)
+        if closed:
+            ops.close()
+        for call in (lambda: ops.lookup(T((9, 4)), I((3,)), T((3, 4))), ops.sync):
+            with pytest.raises(ValueError, match="null context"):
+                call()
