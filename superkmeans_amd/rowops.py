@@ -17,6 +17,9 @@ the object was made with.
 
 Shapes, types, layouts and devices are checked on the host (ValueError, TypeError); indices are not, and one that points
 outside of its table stands for no row.
+
+torch's wheel carries a HIP runtime of its own, and the first one that a process loads has to serve both: import torch before
+this package (tensors of a torch that came later are refused with a RuntimeError).
 """
 import ctypes
 
@@ -34,6 +37,14 @@ def _dtype_name(dtype):
     return str(dtype).rsplit(".", 1)[-1]
 
 
+def _one_runtime():
+    """Refuses tensors of a torch that came with a second HIP runtime: streams and memory of one mean nothing to the other."""
+    with open("/proc/self/maps") as maps:
+        found = {line.split(None, 5)[5].rstrip("\n") for line in maps if "/libamdhip64.so" in line}
+    if len(found) > 1:
+        raise RuntimeError(f"two HIP runtimes are loaded ({', '.join(sorted(found))}): import torch before superkmeans_amd")
+
+
 class _Kinds(dict):
     """dtype object -> code of the C interface, for the types that an argument may have; filled as dtypes come along."""
 
@@ -42,6 +53,8 @@ class _Kinds(dict):
         self.codes = codes
 
     def __missing__(self, dtype):
+        if type(dtype).__module__.partition(".")[0] == "torch":
+            _one_runtime()
         name = _dtype_name(dtype)
         if name not in self.codes:
             raise TypeError(f"must be {' or '.join(self.codes)}, not {name}")

@@ -332,3 +332,38 @@ def test_a_closed_context_is_not_used_again(capi):
         for call in (lambda: ops.lookup(T((9, 4)), I((3,)), T((3, 4))), ops.sync):
             with pytest.raises(ValueError, match="null context"):
                 call()
+
+
+IMPORTS = {
+    "torch first": "import torch; from superkmeans_amd import _capi; _capi.load()",
+    "torch later": "from superkmeans_amd import _capi; _capi.load(); import torch",
+}
+
+
+@pytest.mark.parametrize("order", sorted(IMPORTS))
+def test_a_second_hip_runtime_is_refused(order):
+    """In processes of their own: what is loaded stays loaded."""
+    import os
+    import subprocess
+    import sys
+
+    program = IMPORTS[order] + """
+import sys
+sys.path.insert(0, "tests")
+from test_rowops_refusals import Context
+from superkmeans_amd.rowops import RowOperators
+runtimes = {line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line}
+x = torch.zeros((2, 4))
+try:
+    RowOperators(ctx=Context()).dispatch(x, torch.zeros((2, 1), dtype=torch.int32), x)
+except (ValueError, RuntimeError) as e:
+    print(len(runtimes), type(e).__name__)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0, r.stderr[-2000:]
+    runtimes, error = r.stdout.split()[-2:]
+    if order == "torch first":
+        assert runtimes == "1"
+    # host tensors: with one runtime they are refused for their device
+    assert error == ("RuntimeError" if int(runtimes) > 1 else "ValueError")
