@@ -602,11 +602,11 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
             }
         }
     };
-    const auto put = [&](const uint32_t r, const uint32_t at, const vec_of<float, E> (&sum)[V]) {
+    const auto put = [&](const uint32_t r, const uint32_t at, const vec_of<float, E> (&sum)[V], const float scale) {
         O* out = reinterpret_cast<O*>(g.out) + (size_t) (r * step + block) * g.out_stride;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (at + i * 64 < g.vectors) put_sum<O, E>(out + column<E>(at + i * 64, g.last), sum[i], g.scale, g.accumulate);
+            if (at + i * 64 < g.vectors) put_sum<O, E>(out + column<E>(at + i * 64, g.last), sum[i], scale, g.accumulate);
     };
     const uint32_t at = blockIdx.y * (64 * V) + lane;  // the workgroup's piece of the rows
     for (uint32_t r = wave; r < mine; r += WAVES) {
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
         vec_of<float, E> sum[V] = {};
         if (tokens)
             for (uint32_t w = 0; w < WAVES; ++w) add_share(w, r, at, sum);
-        put(r, at, sum);
+        put(r, at, sum, tokens ? g.scale : 1.0f);  // zeros whatever the scale
     }
     for (uint32_t r = 0; r < mine; ++r) {
         if (of_row[r] <= FEW_MOST) continue;
@@ -628,7 +628,7 @@ __global__ __launch_bounds__(FEW_THREADS) void lookup_grad_few_kernel(const Grad
             for (int w = 1; w < WAVES; ++w)
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += share[w][i][lane];
-            put(r, at, sum);
+            put(r, at, sum, g.scale);
         }
         __syncthreads();
     }

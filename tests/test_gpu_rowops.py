@@ -1100,3 +1100,19 @@ def test_arrays_know_their_device(capi, ctx, ops):
     assert km.ctx.device == 0
     km.close()
     a.free()
+
+
+@pytest.mark.parametrize("scale", [-1.0, np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("n", [5, 3000])
+def test_rows_without_a_token_are_zeros_whatever_the_scale(dev, ops, n, scale):
+    """Zeros are stored, not a product of zero and the scale: neither NaN nor -0."""
+    rows, d = 40, 12
+    ids = np.arange(n) % 3 * 11 + 2
+    for kind in KINDS:
+        out = dev(np.full((rows, d), 5), kind)
+        ops.lookup_grad(dev(np.ones((n, d)), kind), dev(ids, "int64"), out, scale=scale)
+        named = np.zeros(rows, bool)
+        named[ids] = True
+        assert np.all(out.raw()[~named].view(np.uint8) == 0)
+        got = out.host()[named]
+        assert np.all(np.isnan(got)) if np.isnan(scale) else np.all(np.sign(got) == np.sign(scale))
