@@ -203,6 +203,12 @@ class RowOperators:
         _capi.check(rc)
 
     @staticmethod
+    def _signed(ids, rows):
+        """Negative 32-bit ids are read as large ones, which are rows of a table of more than 2^31."""
+        if rows > 1 << 31 and _dtype_name(ids.dtype) == "int32":
+            raise ValueError(f"ids of int32 cannot point into {rows} rows")
+
+    @staticmethod
     def _misfit(what, has, wants):
         raise ValueError(f"{what} must have shape {wants}, not {has}")
 
@@ -215,7 +221,8 @@ class RowOperators:
     def lookup(self, table, ids, out, scale=1.0):
         """out[t] = scale * table[ids[t]], zeros where the id is no row.
 
-        table : (rows, d) float32, float16 or bfloat16;  ids : (n,) int32, uint32 or int64;  out : (n, d) of the table's type.
+        table : (rows, d) float32, float16 or bfloat16;  ids : (n,) int32 (up to 2^31 rows), uint32 or int64;  out : (n, d) of the
+        table's type.
         """
         table_at, kind, rows, d, table_stride = self._matrix(table, "table", _VALUES)
         ids_at, ids_kind, n = self._vector(ids, "ids", _IDS)
@@ -224,6 +231,7 @@ class RowOperators:
             self._same_kind("out", out_kind, "table")
         if out_rows != n or out_d != d:
             self._misfit("out", (out_rows, out_d), (n, d))
+        self._signed(ids, rows)
         self._call(self._lib.skm_lookup_rows(self._handle, table_at, kind, rows, d, table_stride, ids_at, ids_kind, n, scale, out_at,
                                              out_stride))
         return out
@@ -244,6 +252,7 @@ class RowOperators:
             self._misfit("ids", (n_ids,), (n,))
         if out_d != d:
             self._misfit("out", (rows, out_d), (rows, d))
+        self._signed(ids, rows)
         scratch_at, scratch_bytes = self._scratch(scratch)
         self._call(self._lib.skm_lookup_rows_grad(self._handle, grad_at, kind, grad_stride, ids_at, ids_kind, n, rows, d, scale, out_at,
                                                   out_kind, out_stride, 1 if accumulate else 0, scratch_at, scratch_bytes))

@@ -367,3 +367,21 @@ except (ValueError, RuntimeError) as e:
         assert runtimes == "1"
     # host tensors: with one runtime they are refused for their device
     assert error == ("RuntimeError" if int(runtimes) > 1 else "ValueError")
+
+
+def test_signed_ids_of_more_rows_than_they_can_name(ops):
+    """-5 in 32 bits is read as 2^32 - 5, a row of a table that long."""
+    many, most = (1 << 31) + 1, 1 << 31
+    calls = [
+        lambda rows, kind: ops.lookup(T((rows, 1)), Tensor((3,), kind), T((3, 1))),
+        lambda rows, kind: ops.lookup_grad(T((3, 1)), Tensor((3,), kind), T((rows, 1))),
+    ]
+    for call in calls:
+        with pytest.raises(ValueError, match="int32"):
+            call(many, "int32")
+    assert ops.ctx.lib.calls == []
+    for call in calls:
+        call(many, "uint32")
+        call(many, "int64")
+        call(most, "int32")
+    assert len(ops.ctx.lib.calls) == 3 * len(calls)
