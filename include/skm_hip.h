@@ -120,7 +120,7 @@ int skm_fill_u32(skm_ctx* ctx, void* d_dst, uint32_t value, size_t count);
 
 /* Per-stage device timers, named like the reference's profiler scopes (profiler.h:296-312;
  * "search/1st_blas", "search/blas", "search/pdx", "rotator", "update_centroids", ...).
- * While enabled every stage brackets its kernels with events on the context's stream. */
+ * While enabled every stage brackets its kernels with events on the context's stream, unless that is being captured. */
 int skm_prof_enable(skm_ctx* ctx, int enabled);
 int skm_prof_reset(skm_ctx* ctx);
 /* Sum of device milliseconds and number of recorded intervals of one scope (synchronises). */

@@ -205,6 +205,14 @@ static hipEvent_t take_event(skm_ctx* ctx) {
 
 ScopedStage::ScopedStage(skm_ctx* ctx, const char* scope) : ctx_(ctx) {
     if (!ctx->prof) return;
+    // A captured call has no time of its own: its events would belong to the graph, and asking for the time between them is
+    // an error that the next launch would be blamed for.
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
+        (void) hipGetLastError();
+        return;
+    }
+    if (status != hipStreamCaptureStatusNone) return;
     iv_.scope = scope;
     iv_.start = take_event(ctx);
     iv_.stop = take_event(ctx);

@@ -98,7 +98,7 @@ int reduction_counter(skm_ctx* ctx, uint32_t** out);
 int host_ring(skm_ctx* ctx, void** out, size_t* out_bytes);
 int pinned_sizes(skm_ctx* ctx, uint32_t** out, size_t* out_entries);
 
-// RAII device timer for one profiler scope; no-op unless profiling is enabled.
+// RAII device timer for one profiler scope; no-op unless profiling is enabled, and under graph capture.
 class ScopedStage {
   public:
     ScopedStage(skm_ctx* ctx, const char* scope);

@@ -1116,3 +1116,35 @@ def test_rows_without_a_token_are_zeros_whatever_the_scale(dev, ops, n, scale):
         assert np.all(out.raw()[~named].view(np.uint8) == 0)
         got = out.host()[named]
         assert np.all(np.isnan(got)) if np.isnan(scale) else np.all(np.sign(got) == np.sign(scale))
+
+
+def test_device_timers_leave_captured_calls_out(hip, dev):
+    """With the timers on, calls are captured and replayed as without; the timers count the eager calls only."""
+    from superkmeans_amd.rowops import RowOperators
+
+    g = np.random.default_rng(2)
+    stream = hip.stream()
+    with RowOperators(device=0, stream=stream.value) as ops:
+        layer = Layer(dev, g, 300, 150, 64, 96, 8, 2, with_scratch_of=ops)
+        ops.ctx.prof_enable()
+        ops.ctx.prof_reset()
+        layer.set(g)
+        layer.run(ops)
+        graph = hip.capture(stream, lambda: layer.run(ops))
+        for _ in range(3):
+            layer.set(g)
+            hip.hipGraphLaunch(graph, stream)
+            ops.sync()
+            layer.check()
+            assert ops.ctx.prof()["rows/route"][1] == 1
+        layer.set(g)
+        layer.run(ops)
+        ops.sync()
+        layer.check()
+        timers = ops.ctx.prof()
+        assert {name: calls for name, (_, calls) in timers.items()} == {
+            f"rows/{name}": 2 for name in ("lookup", "route", "dispatch", "quantize", "product", "combine", "combine_grad", "lookup_grad")}
+        assert all(ms > 0 for ms, _ in timers.values())
+        ops.ctx.prof_enable(False)
+        hip.hipGraphExecDestroy(graph)
+    hip.hipStreamDestroy(stream)
