@@ -13,16 +13,16 @@ own = False
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 IDS = {"u32": torch.int32, "i64": torch.int64}  # a 32-bit id is read as unsigned: -1 stands for 0xffffffff
 
-_operators = None
+_operators = {}  # by stream
 
 
 def _own_operators():
-    global _operators
-    if _operators is None:
+    stream = torch.cuda.current_stream().cuda_stream
+    if stream not in _operators:
         from superkmeans_amd.rowops import RowOperators
 
-        _operators = RowOperators(device=0, stream=torch.cuda.current_stream().cuda_stream)
-    return _operators
+        _operators[stream] = RowOperators(device=0, stream=stream)
+    return _operators[stream]
 
 
 # --------------------------------------------------------------------------------------------------------------------
