@@ -1148,3 +1148,43 @@ def test_device_timers_leave_captured_calls_out(hip, dev):
         ops.ctx.prof_enable(False)
         hip.hipGraphExecDestroy(graph)
     hip.hipStreamDestroy(stream)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# long rows of a gradient, exactly
+# ---------------------------------------------------------------------------------------------------------------------
+
+# Gradients of whole numbers from 1 to 8, sums below 2^24: fp32 adds them exactly in any order, so results have to be equal, and as
+# every token adds something to every column, none can be lost unseen.
+WHOLE = [(2100, 3, 257, "one"), (2500, 7, 600, "text"), (40000, 2049, 20, "one"), (40000, 2049, 20, "two runs"), (40000, 2049, 20, "even"),
+         (131072, 11, 9, "two runs"), (140000, 500, 5, "one"), (140000, 500, 5, "text"), (500000, 4, 33, "even"), (1048577, 1, 3, "one"),
+         (1100000, 40, 2, "text"), (1100000, 40, 2, "two runs"), (1100000, 70001, 3, "even"), (1100000, 70001, 3, "one")]
+
+
+def whole_case(n, rows, d, how):
+    """(grad, ids, sums) in whole numbers."""
+    g = np.random.default_rng(n + rows + d)
+    grad, ids = g.integers(1, 9, (n, d)), spread_ids(g, n, rows, how)
+    there = (ids >= 0) & (ids < rows)
+    sums = np.stack([np.bincount(ids[there], weights=column[there], minlength=rows) for column in grad.T], 1)
+    assert sums.max() < 1 << 24
+    return grad, ids, sums
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n,rows,d,how", WHOLE)
+def test_lookup_grad_of_whole_numbers(dev, ops, kind, n, rows, d, how):
+    grad, ids, sums = whole_case(n, rows, d, how)
+    on_device, held = dev(grad, kind), np.arange(rows * d).reshape(rows, d) % 100
+    for ids_kind, scale in (("int64", 1.0), ("int32", -0.5)):
+        where = dev(ids, ids_kind)
+        out = dev(np.full((rows, d), 5), "float32")
+        ops.lookup_grad(on_device, where, out, scale=scale)
+        assert np.array_equal(out.host(), sums * scale)
+        out = dev(held, "float32")
+        ops.lookup_grad(on_device, where, out, scale=scale, accumulate=True)
+        assert np.array_equal(out.host(), sums * scale + held)
+        if kind != "float32":
+            out = dev(np.full((rows, d), 5), kind)
+            ops.lookup_grad(on_device, where, out, scale=scale)
+            assert np.array_equal(out.host(), typed(sums * scale, kind))  # one rounding of the exact sum
