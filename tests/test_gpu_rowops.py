@@ -956,7 +956,7 @@ class Block:
         self.capi, self.ctx, self.shape, self.dtype, self.kind = capi, ctx, shape, kind, kind
         size = int(np.prod(shape, dtype=np.int64))
         self.raw_type = np.dtype(RAW.get(kind, kind))
-        self.memory = ctx.empty(size + 4, self.raw_type)
+        self.memory = ctx.empty((size + 7) // 4 * 4, self.raw_type)  # whole words, some behind the last element
         capi.check(ctx.lib.skm_fill_u32(ctx.handle, self.memory.ptr, word, self.memory.nbytes // 4))
 
     def stride(self):
@@ -1188,3 +1188,106 @@ def test_lookup_grad_of_whole_numbers(dev, ops, kind, n, rows, d, how):
             out = dev(np.full((rows, d), 5), kind)
             ops.lookup_grad(on_device, where, out, scale=scale)
             assert np.array_equal(out.host(), typed(sums * scale, kind))  # one rounding of the exact sum
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# variants that only some sizes choose
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kind,d", [("float16", 24), ("float32", 100), ("bfloat16", 257), ("float32", 7), ("bfloat16", 2056), ("float32", 1024)])
+@pytest.mark.parametrize("rest", [0, 1, 2, 3])
+def test_lookup_of_so_many_rows_that_wavefronts_take_four(dev, block, ops, kind, d, rest):
+    """From 32,768 wavefronts of work on each takes four times its rows: those of a last, partly filled one among them."""
+    elements = min(16 // (4 if kind == "float32" else 2), d)
+    elements = 1 << (elements.bit_length() - 1)
+    vectors, lanes = -(-d // elements), 1
+    while lanes < 64 and lanes * 4 < vectors:
+        lanes *= 2
+    pieces = -(-vectors // (4 * lanes))
+    n = 32768 // pieces * (64 // lanes) + 4 * (64 // lanes) * 5 + rest * (64 // lanes) + rest
+    g = np.random.default_rng(n)
+    rows = 1000
+    table, ids = typed(g.standard_normal((rows, d)), kind), g.integers(-1, rows + 1, n)
+    on_device, where, out = dev(table, kind, 3), dev(ids, "int32"), block((n, d), kind, 0x01010101)
+    there = (ids >= 0) & (ids < rows)
+    for scale in (1.0, -0.5):
+        ops.lookup(on_device, where, out, scale=scale)
+        want = encode(np.concatenate([table * scale, np.zeros((1, d))]), kind)[np.where(there, ids, rows)]
+        got = out.memory.download()
+        assert np.array_equal(got[: n * d].reshape(n, d).view(np.uint8), want.view(np.uint8))
+        assert np.all(got[n * d:].view(np.uint8) == 1)  # nothing behind the last row
+
+
+@pytest.mark.parametrize("kind,out_kind", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("d", [300, 301, 500, 512, 516, 768, 900, 1100, 2047])
+def test_lookup_grad_of_few_tokens_on_wide_rows(dev, ops, kind, out_kind, d):
+    """Rows of up to 64, 128, 192 and more vectors, alone and with more than eight tokens, stored and accumulated, exactly."""
+    g = np.random.default_rng(d)
+    for n, rows in ((1021, 200), (2048, 64), (250, 3)):
+        grad, ids = g.integers(1, 9, (n, d)), spread_ids(g, n, rows, "text")
+        held = g.integers(-50, 50, (rows, d))
+        there = (ids >= 0) & (ids < rows)
+        sums = np.zeros((rows, d))
+        np.add.at(sums, ids[there], grad[there])
+        counts = np.bincount(ids[there], minlength=rows)
+        assert counts.max() > 8 and (rows < 10 or counts.min() <= 8)
+        on_device, where = dev(grad, kind, 5), dev(ids, "int64")
+        out = dev(np.full((rows, d), 5), out_kind, 1)
+        ops.lookup_grad(on_device, where, out)
+        assert np.array_equal(out.host(), typed(sums, out_kind)) and out.margin_untouched()
+        out = dev(held, out_kind, 1)
+        ops.lookup_grad(on_device, where, out, accumulate=True)
+        assert np.array_equal(out.host(), typed(sums + held, out_kind)) and out.margin_untouched()
+
+
+@pytest.mark.parametrize("out_kind", KINDS)
+@pytest.mark.parametrize("m,n,k,sizes", [(2047, 4095, 272, None), (2048, 4096, 128, None), (2000, 4095, 144, [700, 0, 513, 780]),
+                                         (2047, 4096, 272, [1, 1023, 900, 123])])
+def test_product_of_tiles_of_128_by_256(dev, ops, out_kind, m, n, k, sizes):
+    """Sizes that give 256 workgroups a tile of 128 x 256, and too few of them one of 256 x 256."""
+    groups = 1 if sizes is None else len(sizes)
+    rows = -(-m // groups)
+    tiles = lambda tm, tn: groups * -(-rows // tm) * -(-n // tn)
+    assert rows > 64 and tiles(256, 256) < 192 and tiles(128, 256) >= 256
+    g = np.random.default_rng(m + k)
+    for pad in (0, 3):
+        a, b = g.integers(-128, 128, (m, k)), g.integers(-128, 128, (groups, n, k))
+        a_scales, b_scales = typed(g.random(m) * 0.01, "float32"), typed(g.random((groups, n)) * 0.01, "float32")
+        bias = typed(g.standard_normal((groups, n)), "float32") if pad else None
+        out = dev(np.full((m, n), 5), out_kind, pad)
+        if sizes is None:
+            ops.product(dev(a, "int8", pad), dev(a_scales, "float32"), dev(b[0], "int8", pad), dev(b_scales[0], "float32"), out,
+                        bias=None if bias is None else dev(bias[0], "float32"))
+            offsets = [0, m]
+        else:
+            offsets = np.concatenate([[0], np.cumsum(sizes)])
+            ops.product(dev(a, "int8", pad), dev(a_scales, "float32"), dev(b, "int8", pad), dev(b_scales, "float32"), out,
+                        bias=None if bias is None else dev(bias, "float32"), offsets=dev(offsets, "int32"))
+        for e in range(groups):
+            i, j = offsets[e], offsets[e + 1]
+            if i < j:
+                want, size = product_of(a[i:j], a_scales[i:j], b[e], b_scales[e], None if bias is None else bias[e])
+                close(out, want, size, 4, rows=slice(i, j))
+        assert np.all(out.host()[offsets[-1]:] == 5) and out.margin_untouched()
+
+
+def test_lookup_of_what_assign_answers(capi, ctx, ops):
+    """The framework's own use: every point replaced by its centroid, and the sums of the points by centroid as the gradient."""
+    g = np.random.default_rng(6)
+    n, k, d = 3001, 37, 48
+    X, C = g.integers(-9, 10, (n, d)).astype(np.float32), g.integers(-9, 10, (k, d)).astype(np.float32)
+    dX, dC = ctx.array(X), ctx.array(C)
+    xn, cn, idx, dist = ctx.empty(n), ctx.empty(k), ctx.empty(n, np.uint32), ctx.empty(n)
+    out, sums, update, sizes = ctx.empty((n, d)), ctx.empty((k, d)), ctx.empty((k, d)), ctx.empty(k, np.uint32)
+    capi.check(ctx.lib.skm_norms(ctx.handle, dX.ptr, n, d, d, xn.ptr))
+    capi.check(ctx.lib.skm_norms(ctx.handle, dC.ptr, k, d, d, cn.ptr))
+    capi.check(ctx.lib.skm_assign_full(ctx.handle, dX.ptr, n, dC.ptr, k, d, xn.ptr, cn.ptr, idx.ptr, dist.ptr))
+    ops.lookup(dC, idx, out)
+    ops.lookup_grad(dX, idx, sums)
+    capi.check(ctx.lib.skm_update(ctx.handle, dX.ptr, n, d, idx.ptr, k, update.ptr, sizes.ptr))
+    assert np.array_equal(out.download(), C[idx.download()])
+    assert np.array_equal(((X - out.download()) ** 2).sum(1), dist.download())  # whole numbers: exact
+    assert np.array_equal(sums.download(), update.download())
+    for a in (dX, dC, xn, cn, idx, dist, out, sums, update, sizes):
+        a.free()
