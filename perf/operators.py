@@ -17,7 +17,7 @@ _operators = {}  # by stream
 
 
 def _own_operators():
-    stream = torch.cuda.current_stream().cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(0)  # current_stream().cuda_stream, which takes as long as half a short call
     if stream not in _operators:
         from superkmeans_amd.rowops import RowOperators
 
