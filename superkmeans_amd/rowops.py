@@ -67,6 +67,13 @@ _IDS = _Kinds({"int32": 3, "uint32": 3, "int64": 4})  # SKM_U32 (a negative 32-b
 _WORDS = _Kinds({"int32": 3, "uint32": 3})
 _STEPS = _Kinds({"int8": 5})
 _F32 = _Kinds({"float32": 0})
+_SIGNED_ROWS = 1 << 31
+
+
+class _Closed:
+    """What an object has in the place of its context once it is closed."""
+
+    handle = None
 
 
 class RowOperators:
@@ -98,17 +105,14 @@ class RowOperators:
         self.device = 0 if device is None else device
         self.ctx = _capi.Context(self.device, stream) if ctx is None else ctx
         self._lib = self.ctx.lib
+        self._context = self.ctx  # its handle is None once it is closed: the library refuses a null context
 
-    @property
-    def _handle(self):
-        """None once the object or the context is closed: the library refuses a null context."""
-        return self.ctx.handle if self.ctx is not None else None
 
     def close(self):
         """Releases the context, if it is the object's own."""
         if self._owned and self.ctx is not None:
             self.ctx.close()
-        self.ctx = None
+        self.ctx, self._context = None, _Closed
 
     def __enter__(self):
         return self
@@ -124,7 +128,7 @@ class RowOperators:
 
     def sync(self):
         """Waits for the stream."""
-        self._call(self._lib.skm_sync(self._handle))
+        self._call(self._lib.skm_sync(self._context.handle))
 
     # -- arguments ---------------------------------------------------------------------------------------------------
     # A decoding step's calls are short: these checks are written for few attribute reads, not for few lines.
@@ -204,8 +208,8 @@ class RowOperators:
 
     @staticmethod
     def _signed(ids, rows):
-        """Negative 32-bit ids are read as large ones, which are rows of a table of more than 2^31."""
-        if rows > 1 << 31 and _dtype_name(ids.dtype) == "int32":
+        """Negative 32-bit ids are read as large ones, which are rows of a table that long."""
+        if _dtype_name(ids.dtype) == "int32":
             raise ValueError(f"ids of int32 cannot point into {rows} rows")
 
     @staticmethod
@@ -231,9 +235,10 @@ class RowOperators:
             self._same_kind("out", out_kind, "table")
         if out_rows != n or out_d != d:
             self._misfit("out", (out_rows, out_d), (n, d))
-        self._signed(ids, rows)
-        self._call(self._lib.skm_lookup_rows(self._handle, table_at, kind, rows, d, table_stride, ids_at, ids_kind, n, scale, out_at,
-                                             out_stride))
+        if rows > _SIGNED_ROWS:
+            self._signed(ids, rows)
+        self._call(self._lib.skm_lookup_rows(self._context.handle, table_at, kind, rows, d, table_stride, ids_at, ids_kind, n,
+                                             scale, out_at, out_stride))
         return out
 
     def lookup_grad(self, grad, ids, out, scale=1.0, accumulate=False, scratch=None):
@@ -252,10 +257,12 @@ class RowOperators:
             self._misfit("ids", (n_ids,), (n,))
         if out_d != d:
             self._misfit("out", (rows, out_d), (rows, d))
-        self._signed(ids, rows)
+        if rows > _SIGNED_ROWS:
+            self._signed(ids, rows)
         scratch_at, scratch_bytes = self._scratch(scratch)
-        self._call(self._lib.skm_lookup_rows_grad(self._handle, grad_at, kind, grad_stride, ids_at, ids_kind, n, rows, d, scale, out_at,
-                                                  out_kind, out_stride, 1 if accumulate else 0, scratch_at, scratch_bytes))
+        self._call(self._lib.skm_lookup_rows_grad(self._context.handle, grad_at, kind, grad_stride, ids_at, ids_kind, n, rows, d,
+                                                  scale, out_at, out_kind, out_stride, 1 if accumulate else 0, scratch_at,
+                                                  scratch_bytes))
         return out
 
     def lookup_grad_scratch(self, n, rows, d):
@@ -286,7 +293,8 @@ class RowOperators:
             if n_order != n * k:
                 self._misfit("order", (n_order,), (n * k,))
         scratch_at, scratch_bytes = self._scratch(scratch)
-        self._call(self._lib.skm_route(self._handle, choices_at, n, k, groups, slots_at, order_at, offsets_at, scratch_at, scratch_bytes))
+        self._call(self._lib.skm_route(self._context.handle, choices_at, n, k, groups, slots_at, order_at, offsets_at, scratch_at,
+                                       scratch_bytes))
         return slots, offsets
 
     def route_scratch(self, n, choices, groups):
@@ -309,7 +317,8 @@ class RowOperators:
             self._misfit("slots", (slots_n, k), (n, k))
         if out_d != d:
             self._misfit("out", (out_rows, out_d), (out_rows, d))
-        self._call(self._lib.skm_dispatch_rows(self._handle, x_at, kind, n, d, x_stride, slots_at, k, out_at, out_rows, out_stride))
+        self._call(self._lib.skm_dispatch_rows(self._context.handle, x_at, kind, n, d, x_stride, slots_at, k, out_at, out_rows,
+                                               out_stride))
         return out
 
     def combine(self, rows, slots, out, weights=None):
@@ -329,8 +338,8 @@ class RowOperators:
             weights_at, weights_kind, weights_n, weights_k = self._dense(weights, "weights", _VALUES)
             if weights_n != n or weights_k != k:
                 self._misfit("weights", (weights_n, weights_k), (n, k))
-        self._call(self._lib.skm_combine_rows(self._handle, rows_at, kind, n_rows, d, rows_stride, slots_at, n, k, weights_at, weights_kind,
-                                              out_at, out_stride))
+        self._call(self._lib.skm_combine_rows(self._context.handle, rows_at, kind, n_rows, d, rows_stride, slots_at, n, k,
+                                              weights_at, weights_kind, out_at, out_stride))
         return out
 
     def combine_grad(self, grad, rows, slots, weights, grad_rows, grad_weights):
@@ -371,8 +380,9 @@ class RowOperators:
             if weights_n != n or weights_k != k:
                 self._misfit("grad_weights", (weights_n, weights_k), (n, k))
             weights_kind = out_kind
-        self._call(self._lib.skm_combine_rows_grad(self._handle, grad_at, kind, n, d, grad_stride, rows_at, n_rows or 0, rows_stride,
-                                                   slots_at, k, weights_at, weights_kind, out_at, out_stride, grad_weights_at))
+        self._call(self._lib.skm_combine_rows_grad(self._context.handle, grad_at, kind, n, d, grad_stride, rows_at, n_rows or 0,
+                                                   rows_stride, slots_at, k, weights_at, weights_kind, out_at, out_stride,
+                                                   grad_weights_at))
         return grad_rows, grad_weights
 
     # -- 8-bit rows --------------------------------------------------------------------------------------------------
@@ -389,7 +399,7 @@ class RowOperators:
             self._misfit("q", (q_n, q_d), (n, d))
         if n_scales != n:
             self._misfit("scales", (n_scales,), (n,))
-        self._call(self._lib.skm_quantize_rows(self._handle, x_at, kind, n, d, x_stride, q_at, q_stride, scales_at))
+        self._call(self._lib.skm_quantize_rows(self._context.handle, x_at, kind, n, d, x_stride, q_at, q_stride, scales_at))
         return q, scales
 
     def product(self, a, a_scales, b, b_scales, out, bias=None, offsets=None):
@@ -441,6 +451,6 @@ class RowOperators:
                     self._misfit("bias", (bias_groups, bias_n), (groups, n))
         if out_m != m or b_n != n or b_k != k or scales_n != n:
             raise ValueError(f"a {(m, k)}, b {(b_n, b_k)}, b_scales of {scales_n} and out {(out_m, n)} do not fit together")
-        self._call(self._lib.skm_product_i8(self._handle, a_at, m, a_stride, a_scales_at, b_at, n, k, b_stride, b_scales_at, bias_at, groups,
-                                            group_stride, offsets_at, out_at, out_kind, out_stride))
+        self._call(self._lib.skm_product_i8(self._context.handle, a_at, m, a_stride, a_scales_at, b_at, n, k, b_stride, b_scales_at,
+                                            bias_at, groups, group_stride, offsets_at, out_at, out_kind, out_stride))
         return out
