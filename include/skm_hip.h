@@ -51,8 +51,8 @@ int skm_device_count(int* out_count);
 int skm_ctx_create(int device, skm_ctx** out_ctx);
 /* The same over a stream of the caller's (a hipStream_t of that device; null: the device's default stream), which has to
  * outlive the context and stays the caller's: work of the context is ordered with the caller's own work on it, and a
- * graph captured on it records the context's launches (the context itself is made before the capture begins: it pins
- * memory).  The calling thread's current device is left as it was.  No counterpart in the reference. */
+ * graph captured on it records the context's launches (the context itself is made before the capture begins, as it pins
+ * memory, and destroyed after it has ended, as that waits for the stream).  The calling thread's current device is left as it was.  No counterpart in the reference. */
 int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx);
 int skm_ctx_destroy(skm_ctx* ctx);
 int skm_ctx_get_device(const skm_ctx* ctx, int* out_device);
@@ -272,7 +272,8 @@ int skm_householder_q(skm_ctx* ctx, const double* h_a, size_t d, float* h_out_q)
  *
  *   - A value type is SKM_F32, SKM_F16 or SKM_BF16.  Sums are held in fp32 and rounded once, to nearest even.
  *   - Matrices are row-major; a stride is the distance between rows in elements, at least the row length.  Any alignment to
- *     the element's size serves; loads are 16 bytes wide where pointers, strides and row lengths allow.
+ *     the element's size serves: rows go in vectors of 16 bytes (of the wider type where two differ) whatever the alignment, in
+ *     narrower ones where a row is shorter or, in an accumulated gradient, no multiple of them.
  *   - Outputs and scratch must not overlap inputs or each other (SKM_ERR_INVALID).  Elements between the rows of a strided output
  *     stay as they are; another matrix of the same stride in bytes may lie there (columns of one buffer), nothing else.
  *   - An index outside the rows it points into stands for no row (SKM_NO_ROW, which skm_knn leaves in empty slots, and
@@ -316,7 +317,8 @@ int skm_lookup_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t grad
 int skm_route_scratch(size_t n, size_t choices, size_t groups, size_t* out_bytes);
 int skm_route(skm_ctx* ctx, const uint32_t* d_choices, size_t n, size_t choices, size_t groups, uint32_t* d_slots,
               uint32_t* d_order, uint32_t* d_offsets, void* d_scratch, size_t scratch_bytes);
-/* out[slots[t][j]] = x[t]: every row copied to its places.  Rows of out (out_rows x d) that are nobody's place stay as they are.
+/* out[slots[t][j]] = x[t]: every row copied to its places, which are distinct, as skm_route makes them (of two rows for one place
+ * either, or parts of both, may be what stays).  Rows of out (out_rows x d) that are nobody's place stay as they are.
  * Its gradient is skm_combine_rows without weights. */
 int skm_dispatch_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t d, size_t x_stride, const uint32_t* d_slots,
                       size_t choices, void* d_out, size_t out_rows, size_t out_stride);
@@ -337,7 +339,8 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
 int skm_quantize_rows(skm_ctx* ctx, const void* d_x, int type, size_t n, size_t d, size_t x_stride, int8_t* d_q, size_t q_stride,
                       float* d_scales);
 /* out[i][j] = (sum over k of a[i][k] b[j][k]) * a_scale[i] * b_scale[j] + bias[j], out (m x n) of out_type; a is m x k, b is n x k.
- * The sum is exact; d_bias may be null.  With d_offsets (groups + 1 entries, as skm_route makes them) the rows
+ * The sum is exact; it is rounded to fp32 and multiplied from left to right, so a product with the first scale that fp32 cannot
+ * hold is an infinity or zero whatever the second scale.  d_bias may be null.  With d_offsets (groups + 1 entries, as skm_route makes them) the rows
  * [offsets[g], offsets[g + 1]) of a are multiplied with the g-th matrix of b (b_group_stride elements apart), b_scale and bias
  * (n apart), and rows of out that are in no group stay as they are.  Without, groups and b_group_stride are not looked at. */
 int skm_product_i8(skm_ctx* ctx, const int8_t* d_a, size_t m, size_t a_stride, const float* d_a_scale, const int8_t* d_b, size_t n,

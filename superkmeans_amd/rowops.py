@@ -18,6 +18,10 @@ the object was made with.
 Shapes, types, layouts and devices are checked on the host (ValueError, TypeError); indices are not, and one that points
 outside of its table stands for no row.
 
+The operators work on memory, beside torch's autograd: a tensor that requires gradients is taken like any other, no graph is
+recorded, and a write into a tensor does not raise its version counter.  Gradients come from the calls named for them, for instance
+in the ``backward`` of a ``torch.autograd.Function``.
+
 torch's wheel carries a HIP runtime of its own, and the first one that a process loads has to serve both: import torch before
 this package (tensors of a torch that came later are refused with a RuntimeError).
 """
@@ -84,8 +88,11 @@ class RowOperators:
     device : int or None
         Device of every tensor that the calls get: 0, or the context's where one is given.
     stream : int or None
-        Handle of the stream to queue on (0: the device's default stream); it has to outlive the object.  None: a stream of
-        the object's own, which callers order with their work through ``sync``.
+        Handle of the stream to queue on (0: the device's default stream); it has to outlive the object.  Give the stream that
+        the tensors are made and used on: work on one stream runs in order, work on two does not.  None: a stream of the
+        object's own.  Nothing makes that wait for work that the caller queued elsewhere, so wait for such work before a call, and
+        ``sync`` before its results are used elsewhere or its tensors are released (the device's default stream and this one
+        wait for each other by themselves; no other stream does).
     ctx : Context or None
         An existing context to work on instead; the object is of no use once that is closed.
 
@@ -306,7 +313,7 @@ class RowOperators:
     def dispatch(self, x, slots, out):
         """out[slots[t, j]] = x[t]; rows of out that are nobody's place stay as they are.
 
-        x : (n, d);  slots : (n, k);  out : (places, d) of x's type.
+        x : (n, d);  slots : (n, k), distinct places as `route` makes them;  out : (places, d) of x's type.
         """
         x_at, kind, n, d, x_stride = self._matrix(x, "x", _VALUES)
         slots_at, _, slots_n, k = self._dense(slots, "slots", _WORDS)
