@@ -370,8 +370,8 @@ int skm_combine_rows_grad(skm_ctx* ctx, const void* d_grad, int type, size_t n, 
                 "strides must be at least d");
     SKM_REQUIRE(n < SKM_NO_ROW && n_rows < SKM_NO_ROW, "row counts must fit in 32 bits");
     SKM_REQUIRE(choices > 0 && choices <= SKM_ROUTE_MAX_CHOICES, "choices out of range");
-    SKM_REQUIRE(d_grad_rows || d_grad_weights, "no output asked for");
     if (n == 0) return SKM_OK;
+    SKM_REQUIRE(d_grad_rows || d_grad_weights, "no output asked for");
     SKM_REQUIRE(d_grad && d_slots && (d_rows || !d_grad_weights || n_rows == 0), "null pointer");
     const size_t size = type_size(type), weight_size = type_size(weights_type);
     SKM_REQUIRE(address(d_slots) % 4 == 0 && address(d_grad) % size == 0 && address(d_rows) % size == 0 &&

@@ -387,6 +387,8 @@ class RowOperators:
             if weights_n != n or weights_k != k:
                 self._misfit("grad_weights", (weights_n, weights_k), (n, k))
             weights_kind = out_kind
+        if n_rows == 0 and grad_weights is None:
+            return grad_rows, grad_weights  # no row to write, and a library may give a tensor of none no address
         self._call(self._lib.skm_combine_rows_grad(self._context.handle, grad_at, kind, n, d, grad_stride, rows_at, n_rows or 0,
                                                    rows_stride, slots_at, k, weights_at, weights_kind, out_at, out_stride,
                                                    grad_weights_at))

@@ -385,3 +385,31 @@ def test_signed_ids_of_more_rows_than_they_can_name(ops):
         call(many, "int64")
         call(most, "int32")
     assert len(ops.ctx.lib.calls) == 3 * len(calls)
+
+
+def test_calls_without_tokens_or_rows_may_have_no_memory(refusing, capi):
+    """Libraries give tensors of no elements no address: nothing to do is no error."""
+    lib, handle, _ = refusing
+
+    class Real(Context):
+        def __init__(self):
+            self.lib, self.handle = lib, handle
+
+    ops = rowops.RowOperators(ctx=Real())
+    empty = lambda shape, kind="float32": Tensor(shape, kind, at=0)
+    ops.lookup(T((9, 4)), empty((0,), "int64"), empty((0, 4)))
+    ops.lookup_grad(empty((0, 4)), empty((0,), "int32"), empty((0, 4)))
+    ops.lookup_grad(empty((0, 4)), empty((0,), "int32"), T((9, 4)), accumulate=True)
+    ops.lookup_grad(T((3, 4)), I((3,)), empty((0, 4)))
+    ops.dispatch(empty((0, 4)), empty((0, 2), "int32"), empty((0, 4)))
+    ops.dispatch(T((3, 4)), I((3, 2)), empty((0, 4)))
+    ops.combine(empty((0, 4)), empty((0, 2), "int32"), empty((0, 4)), weights=empty((0, 2)))
+    ops.combine_grad(empty((0, 4)), empty((0, 4)), empty((0, 2), "int32"), empty((0, 2)), empty((0, 4)), empty((0, 2)))
+    ops.combine_grad(empty((0, 4)), None, empty((0, 2), "int32"), None, empty((0, 4)), None)
+    ops.combine_grad(empty((0, 4)), empty((0, 4)), empty((0, 2), "int32"), None, None, empty((0, 2)))
+    ops.combine_grad(T((3, 4)), None, I((3, 2)), T((3, 2)), empty((0, 4)), None)
+    ops.quantize(empty((0, 4)), empty((0, 4), "int8"), empty((0,)))
+    ops.product(empty((0, 8), "int8"), empty((0,)), q8((5, 8)), T((5,)), empty((0, 5)))
+    ops.product(empty((0, 8), "int8"), empty((0,)), q8((2, 5, 8)), T((2, 5)), empty((0, 5)), offsets=I((3,)))
+    with pytest.raises(ValueError, match="no output"):
+        ops.combine_grad(T((3, 4)), T((6, 4)), I((3, 2)), T((3, 2)), None, None)
