@@ -296,6 +296,16 @@ static int create_context(int device, bool own_stream, void* stream, skm_ctx** o
         return set_error(SKM_ERR_INVALID, "skm_ctx_create: device %d out of range [0,%d)", device, n);
     const DeviceAsItWas as_it_was(!own_stream);
     SKM_HIP_TRY(hipSetDevice(device));
+    if (!own_stream) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        SKM_HIP_TRY(hipStreamIsCapturing((hipStream_t) stream, &status));
+        if (status != hipStreamCaptureStatusNone)
+            return set_error(SKM_ERR_INVALID, "skm_ctx_create_on_stream: the stream is being captured");
+        hipDevice_t of_stream = device;
+        SKM_HIP_TRY(hipStreamGetDevice((hipStream_t) stream, &of_stream));
+        if (of_stream != device)
+            return set_error(SKM_ERR_INVALID, "skm_ctx_create_on_stream: a stream of device %d for a context on device %d", of_stream, device);
+    }
     hipDeviceProp_t prop;
     SKM_HIP_TRY(hipGetDeviceProperties(&prop, device));
     if (strncmp(prop.gcnArchName, "gfx950", 6) != 0)

@@ -1291,3 +1291,23 @@ def test_lookup_of_what_assign_answers(capi, ctx, ops):
     assert np.array_equal(sums.download(), update.download())
     for a in (dX, dC, xn, cn, idx, dist, out, sums, update, sizes):
         a.free()
+
+
+def test_no_context_is_made_on_a_capturing_stream(hip, dev, capi):
+    """The refusal leaves the capture in working order."""
+    from superkmeans_amd.rowops import RowOperators
+
+    stream = hip.stream()
+    few, slots, offsets = dev(np.ones((4, 2)), "int32"), dev(np.zeros((4, 2)), "int32"), dev(np.zeros(9), "int32")
+    with RowOperators(device=0, stream=stream.value) as ops:
+        def work():
+            with pytest.raises(capi.SkmError, match="captured"):
+                RowOperators(device=0, stream=stream.value)
+            ops.route(few, 8, slots, offsets)
+
+        graph = hip.capture(stream, work)
+        hip.hipGraphLaunch(graph, stream)
+        ops.sync()
+        assert np.array_equal(offsets.raw(), [0, 0] + [8] * 7)
+        hip.hipGraphExecDestroy(graph)
+    hip.hipStreamDestroy(stream)
