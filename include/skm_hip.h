@@ -53,7 +53,9 @@ int skm_ctx_create(int device, skm_ctx** out_ctx);
  * outlive the context and stays the caller's: work of the context is ordered with the caller's own work on it, and a
  * graph captured on it records the context's launches (the context itself is made before the capture begins, as it pins
  * memory: SKM_ERR_INVALID on a capturing stream, or one of another device; and destroyed after it has ended, as that waits for
- * the stream).  The calling thread's current device is left as it was.  No counterpart in the reference. */
+ * the stream).  The calling thread's current device is left as it was.  The default stream belongs to the device that is current: over
+ * it, the entries other than skm_sync, the timers and the operators on rows want the context's device to be current.  No counterpart
+ * in the reference. */
 int skm_ctx_create_on_stream(int device, void* stream, skm_ctx** out_ctx);
 int skm_ctx_destroy(skm_ctx* ctx);
 int skm_ctx_get_device(const skm_ctx* ctx, int* out_device);

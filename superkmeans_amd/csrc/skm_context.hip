@@ -16,6 +16,21 @@ namespace skm {
 
 static thread_local char g_last_error[512] = "";
 
+// Puts the calling thread's device back: a caller that brings its own stream has work of its own on some device.
+class DeviceAsItWas {
+  public:
+    explicit DeviceAsItWas(const bool put_back) : known_(put_back && hipGetDevice(&device_) == hipSuccess) {}
+    ~DeviceAsItWas() {
+        if (known_) (void) hipSetDevice(device_);
+    }
+    DeviceAsItWas(const DeviceAsItWas&) = delete;
+    DeviceAsItWas& operator=(const DeviceAsItWas&) = delete;
+
+  private:
+    int device_ = 0;
+    bool known_;
+};
+
 int set_error(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
@@ -192,6 +207,14 @@ int reduction_counter(skm_ctx* ctx, uint32_t** out) {
     return SKM_OK;
 }
 
+// A caller's stream may be the default one, which belongs to the current device.
+static int wait_for_stream(skm_ctx* ctx) {
+    const DeviceAsItWas as_it_was(!ctx->owns_stream);
+    if (!ctx->owns_stream) SKM_HIP_TRY(hipSetDevice(ctx->device));
+    SKM_HIP_TRY(hipStreamSynchronize(ctx->stream));
+    return SKM_OK;
+}
+
 static hipEvent_t take_event(skm_ctx* ctx) {
     if (!ctx->event_pool.empty()) {
         hipEvent_t e = ctx->event_pool.back();
@@ -230,7 +253,7 @@ ScopedStage::~ScopedStage() {
 
 int resolve_pending(skm_ctx* ctx) {
     if (ctx->pending.empty()) return SKM_OK;
-    SKM_HIP_TRY(hipStreamSynchronize(ctx->stream));
+    SKM_TRY(wait_for_stream(ctx));
     for (auto& iv : ctx->pending) {
         float ms = 0.0f;
         if (hipEventElapsedTime(&ms, iv.start, iv.stop) == hipSuccess) {
@@ -270,21 +293,6 @@ int skm_device_count(int* out_count) {
     *out_count = n;
     return SKM_OK;
 }
-
-// Puts the calling thread's device back: a caller that brings its own stream has work of its own on some device.
-class DeviceAsItWas {
-  public:
-    explicit DeviceAsItWas(const bool put_back) : known_(put_back && hipGetDevice(&device_) == hipSuccess) {}
-    ~DeviceAsItWas() {
-        if (known_) (void) hipSetDevice(device_);
-    }
-    DeviceAsItWas(const DeviceAsItWas&) = delete;
-    DeviceAsItWas& operator=(const DeviceAsItWas&) = delete;
-
-  private:
-    int device_ = 0;
-    bool known_;
-};
 
 static int create_context(int device, bool own_stream, void* stream, skm_ctx** out_ctx) {
     if (!out_ctx) return set_error(SKM_ERR_INVALID, "skm_ctx_create: null output");
@@ -382,8 +390,7 @@ int skm_ctx_destroy(skm_ctx* ctx) {
 
 int skm_sync(skm_ctx* ctx) {
     SKM_REQUIRE(ctx, "null context");
-    SKM_HIP_TRY(hipStreamSynchronize(ctx->stream));
-    return SKM_OK;
+    return wait_for_stream(ctx);
 }
 
 int skm_ctx_set_workspace_limit(skm_ctx* ctx, size_t bytes) {
