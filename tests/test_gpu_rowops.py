@@ -1311,3 +1311,80 @@ def test_no_context_is_made_on_a_capturing_stream(hip, dev, capi):
         assert np.array_equal(offsets.raw(), [0, 0] + [8] * 7)
         hip.hipGraphExecDestroy(graph)
     hip.hipStreamDestroy(stream)
+
+
+def test_two_threads_with_an_object_each(hip, ctx):
+    """Calls at the same time on two streams, with workspaces that grow meanwhile."""
+    import threading
+
+    from superkmeans_amd import _capi
+    from superkmeans_amd.rowops import RowOperators
+
+    failures = []
+
+    def work(seed):
+        try:
+            stream = hip.stream()
+            mine = _capi.Context(0)
+            made = []
+
+            def make(x, kind, pad=0):
+                made.append(Device(mine, x, kind, pad))
+                return made[-1]
+
+            g = np.random.default_rng(seed)
+            with RowOperators(device=0, stream=stream.value) as ops:
+                for n in (40, 3000, 9000, 500, 12000):
+                    layer = Layer(make, g, n, 150, 64, 96, 8, 2)
+                    for _ in range(2):
+                        layer.set(g)
+                        layer.run(ops)
+                        ops.sync()
+                        layer.check()
+            mine.close()
+            hip.hipStreamDestroy(stream)
+        except BaseException as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(100)
+    assert not failures, failures
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, "tests")
+import numpy as np
+from superkmeans_amd import _capi
+from superkmeans_amd.rowops import RowOperators
+from test_gpu_rowops import Device, Hip, Layer
+ctx, hip = _capi.Context(0), Hip()
+made = []
+def dev(x, kind, pad=0):
+    made.append(Device(ctx, x, kind, pad))
+    return made[-1]
+g = np.random.default_rng(0)
+stream = hip.stream()
+with RowOperators(device=0, stream=stream.value) as ops:
+    layer = Layer(dev, g, 9000, 150, 64, 96, 8, 2, with_scratch_of=ops)
+    graph = hip.capture(stream, lambda: layer.run(ops))
+    for _ in range(3):
+        layer.set(g)
+        hip.hipGraphLaunch(graph, stream)
+        ops.sync()
+        layer.check()
+    layer.set(g)
+    layer.run(ops)
+    ops.sync()
+    layer.check()
+print("first calls: ok")
+"""
+
+
+def test_the_first_calls_of_a_process_may_be_captured():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "first calls: ok" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
