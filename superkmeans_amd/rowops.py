@@ -31,9 +31,6 @@ import numpy as np
 
 from . import _capi
 
-_SIZES = {"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "uint32": 4, "int64": 8, "int8": 1, "uint8": 1}
-
-
 def _dtype_name(dtype):
     """"float32" for numpy's and torch's float32 alike."""
     if isinstance(dtype, (np.dtype, type)):
@@ -71,6 +68,7 @@ _IDS = _Kinds({"int32": 3, "uint32": 3, "int64": 4})  # SKM_U32 (a negative 32-b
 _WORDS = _Kinds({"int32": 3, "uint32": 3})
 _STEPS = _Kinds({"int8": 5})
 _F32 = _Kinds({"float32": 0})
+_SCRATCH = _Kinds({"float32": 4, "float16": 2, "bfloat16": 2, "int32": 4, "uint32": 4, "int64": 8, "int8": 1, "uint8": 1})  # sizes
 _SIGNED_ROWS = 1 << 31
 
 
@@ -200,11 +198,8 @@ class RowOperators:
             return None, 0
         if not hasattr(scratch, "dtype"):
             raise TypeError(f"scratch must be a device tensor, not {type(scratch).__name__}")
-        name = _dtype_name(scratch.dtype)
-        if name not in _SIZES:
-            raise TypeError(f"scratch cannot be of {name}")
-        at, _, n = self._vector(scratch, "scratch", _Kinds({name: 0}))
-        return at, n * _SIZES[name]
+        at, size, n = self._vector(scratch, "scratch", _SCRATCH)
+        return at, n * size
 
     def _call(self, rc):
         if rc == 0:

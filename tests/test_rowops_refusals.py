@@ -413,3 +413,33 @@ def test_calls_without_tokens_or_rows_may_have_no_memory(refusing, capi):
     ops.product(empty((0, 8), "int8"), empty((0,)), q8((2, 5, 8)), T((2, 5)), empty((0, 5)), offsets=I((3,)))
     with pytest.raises(ValueError, match="no output"):
         ops.combine_grad(T((3, 4)), T((6, 4)), I((3, 2)), T((3, 2)), None, None)
+
+
+def test_the_process_s_libraries_are_looked_at_once_per_type(ops, monkeypatch):
+    """Not for every call: that takes about as long as a hundred of them."""
+    looks = []
+    monkeypatch.setattr(rowops, "_one_runtime", lambda: looks.append(1))
+
+    class Type:
+        def __init__(self, name):
+            self.name = name
+
+        def __str__(self):
+            return f"torch.{self.name}"
+
+    Type.__module__ = "torch"
+    kinds = {name: Type(name) for name in ("float32", "int64", "uint8")}
+
+    def tensor(shape, kind):
+        t = Tensor(shape, kind)
+        t.dtype = kinds[kind]
+        return t
+
+    for call in range(3):
+        ops.lookup_grad(tensor((3, 4), "float32"), tensor((3,), "int64"), tensor((9, 4), "float32"), scratch=tensor((4096,), "uint8"))
+        if call == 0:
+            first = len(looks)
+    assert 0 < first == len(looks)
+    assert ops.ctx.lib.calls[-1][1][-1] == 4096
+    with pytest.raises(TypeError, match="scratch"):
+        ops.lookup_grad(T((3, 4)), I((3,)), T((9, 4)), scratch=Tensor((64,), "float64"))
