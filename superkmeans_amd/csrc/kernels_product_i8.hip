@@ -19,8 +19,8 @@ typedef int intx16 __attribute__((ext_vector_type(16)));
 
 // The whole numbers nearest to 127 x / most, ties to even, as bytes.  The fp32 product of x and the rounded 127 / most is at most
 // 127 * (2^-23 + 2^-48) < 1.52e-5 off, so that the choice between two numbers can only be wrong that near to the border between
-// them; there the quotient is taken in fp64, where 127 x is exact and a quotient of two fp32 numbers cannot round onto a border.  Adding
-// 1.5 * 2^23 rounds an fp32 number of that size to a whole one, whose last byte is the step.
+// them; there the quotient is taken in fp64, where 127 x is exact and a quotient of two fp32 numbers cannot round onto a border.
+// Adding 1.5 * 2^23 rounds an fp32 number of that size to a whole one, whose last byte is the step.
 template <int E>
 __device__ __forceinline__ vec_of<int8_t, E> nearest_steps(const vec_of<float, E> x, const float most, const float inverse) {
     uint32_t step[E];
